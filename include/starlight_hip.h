@@ -322,6 +322,81 @@ sl_status sl_hip_paged_store(sl_hip_device *device, const sl_paged_kv *kv, uint3
                              uint32_t index, uint32_t max_seq, uint32_t kv_heads, uint32_t head_dim,
                              uint32_t length);
 
+/* The new tokens of one serving step over a paged cache, any number per row
+ * (no reference counterpart: gaps G-17 / G-18, ARCH-0008:123-124). All rows'
+ * tokens lie one after the other; `row_starts` (u32, batch + 1 words or more, at
+ * most 16 MiB) holds each row's first: row b's are row_starts[b] ..
+ * row_starts[b + 1] - 1, rising from 0 to `tokens`; a row may have none. The
+ * i-th token of row b sits at position seq_lens[b] + i. */
+typedef struct sl_paged_tokens {
+    uint32_t batch;
+    uint32_t tokens;
+    uint32_t row_starts;
+    uint32_t reserved;
+} sl_paged_tokens;
+
+/* A block-table entry of a position range whose page has been given back (say,
+ * behind a sliding window): never read. */
+#define SL_PAGE_NONE 4294967295u
+
+/* The three operators below serve such a step, layer by layer: append rotates
+ * and stores the new keys and values, then one of the two attentions reads them.
+ * `op` is the layer's CausalAttention op (layer, heads, kv_heads, head_dim, scale;
+ * head_dim a multiple of 16 up to 256, any number of query heads per KV head);
+ * q, k, v and outputs are token-major, [tokens, heads, head_dim] and [tokens,
+ * kv_heads, head_dim], f32 at any offset, as projections write and read them.
+ * The tables, lengths and row starts are checked on the host from the last
+ * upload_u32. Each call submits the logged commands first and enqueues its
+ * kernels at once on the device's stream, without allocating; the attentions'
+ * partial results use the device workspace, so that work captured from one
+ * device's stream must not run beside its other work. Captured and replayed, a
+ * call reads the tables, lengths and row starts as they then are: they must
+ * still satisfy what is said here, with the same number of tokens. seq_lens is
+ * not advanced: the caller adds each row's tokens after the step. Errors beside
+ * those named: UnsupportedOp for another op code; Unimplemented for a head_dim
+ * or page_size not named here, buffers above 16 MiB, or a block table of more
+ * than 2^31 - 1 positions; Execution for shapes, lengths, row starts, page ids
+ * or aliases that do not fit; InvalidBuffer and InvalidRange as dispatch. A
+ * refused call changes nothing. */
+
+/* Stores the new keys and values k and v at their positions in layer op->layer
+ * of the cache, the keys rotated as the Rope op `rope` (variant, theta) rotates
+ * them at those positions, or as they are when rope is null. q and q_out, both
+ * or neither: the queries, rotated the same way. Rotated values equal the Rope
+ * operator's bit for bit. Execution when a page that a row appends into is also
+ * another row's, or twice the row's own. */
+sl_status sl_hip_paged_append(sl_hip_device *device, const sl_op *op, const sl_op *rope, const sl_buffer_ref *q,
+                              const sl_buffer_ref *k, const sl_buffer_ref *v, const sl_buffer_ref *q_out,
+                              const sl_paged_tokens *tokens, const sl_paged_kv *kv);
+
+/* Attention of every new token over its row's pages, the step's own positions
+ * (already appended) included: a token at position p sees the positions j <= p
+ * with j > p - window or j < sinks; window 0 is no window, and sinks is then not
+ * read. Pages without a position that a token of the call sees are not read, and
+ * their table entries may be anything. */
+sl_status sl_hip_paged_window_attention(sl_hip_device *device, const sl_op *op, const sl_buffer_ref *q,
+                                        const sl_buffer_ref *out, uint32_t window, uint32_t sinks,
+                                        const sl_paged_tokens *tokens, const sl_paged_kv *kv);
+
+/* The same attention, without a window, for rows whose tables begin with the same
+ * pages for positions 0 .. prefix - 1 (a common prompt): those keys and values
+ * are read once for all rows instead of once per row. Execution when a row with
+ * tokens has fewer cached positions than the prefix or other pages there; rows
+ * without tokens are not looked at. */
+sl_status sl_hip_paged_prefix_attention(sl_hip_device *device, const sl_op *op, const sl_buffer_ref *q,
+                                        const sl_buffer_ref *out, uint32_t prefix, const sl_paged_tokens *tokens,
+                                        const sl_paged_kv *kv);
+
+/* The device address of f32 buffer `buffer`, valid until the device is destroyed,
+ * and, where `elements` is not null, its capacity: for a program that makes or reads its contents with kernels of its own, or hands
+ * them to another library without a copy (no reference counterpart). Logged
+ * commands are submitted first; accesses are ordered with the device's work as any
+ * other on sl_hip_stream's device are (on that stream, or synchronized). Writing
+ * the scales of a bound quantized weight this way does not refresh its copies.
+ * InvalidBuffer for a u32 buffer, whose contents the device also keeps on the
+ * host; a null address for a buffer of no elements. */
+sl_status sl_hip_buffer_address(sl_hip_device *device, uint32_t buffer, void **out, uint64_t *elements);
+
 /* One entry of the buffer table sl_hip_validate_dispatch checks against. */
 typedef enum sl_buffer_kind {
     SL_BUFFER_NONE = 0,
@@ -350,6 +425,21 @@ sl_status sl_hip_validate_dispatch(const sl_buffer_desc *buffers, size_t n_buffe
                                    size_t n_inputs, const sl_buffer_ref *outputs,
                                    const sl_value *output_values, size_t n_outputs,
                                    const uint32_t *scalars, size_t n_scalars, sl_error *err);
+
+/* The operators on ragged new tokens, for sl_hip_validate_paged. */
+typedef enum sl_paged_kind { SL_PAGED_APPEND = 0, SL_PAGED_WINDOW = 1, SL_PAGED_PREFIX = 2 } sl_paged_kind;
+
+/* Validation only, no GPU needed: the checks that the paged operator `kind`
+ * makes before it enqueues anything, against a caller-described buffer table
+ * indexed by buffer id and host copies of the three u32 buffers (row_starts:
+ * batch + 1 words, seq_lens: batch, block_table: batch * pages_per_seq). Ports
+ * that the operator lacks (rope, k and v but for append) are null; `window` is
+ * append's 0, the window's or the prefix, `sinks` the window's. */
+sl_status sl_hip_validate_paged(const sl_buffer_desc *buffers, size_t n_buffers, uint32_t kind, const sl_op *op,
+                                const sl_op *rope, const sl_buffer_ref *q, const sl_buffer_ref *k,
+                                const sl_buffer_ref *v, const sl_buffer_ref *out, uint32_t window, uint32_t sinks,
+                                const sl_paged_tokens *tokens, const sl_paged_kv *kv, const uint32_t *row_starts,
+                                const uint32_t *seq_lens, const uint32_t *block_table, sl_error *err);
 
 /* sl_ir::DeviceCapabilities (ARCH-0004 §8) for this backend; op masks are
  * bitsets over sl_opcode. Consumed by the graph compiler, not by dispatch. */

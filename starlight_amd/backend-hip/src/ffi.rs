@@ -52,6 +52,12 @@ pub const SL_ENCODING_OPAQUE_QUANTIZED: u32 = 2;
 pub const SL_QFORMAT_INT4: u32 = 0;
 pub const SL_QFORMAT_INT8: u32 = 1;
 
+/// `sl_paged_kind`: the operators on ragged new tokens.
+pub const SL_PAGED_APPEND: u32 = 0;
+pub const SL_PAGED_WINDOW: u32 = 1;
+pub const SL_PAGED_PREFIX: u32 = 2;
+pub const SL_PAGE_NONE: u32 = 4294967295;
+
 /// `sl_opcode` (sl_ir::OpCode declaration order, ARCH-0004 §5.1).
 pub const SL_OP_MATMUL_NT: u32 = 0;
 pub const SL_OP_MATMUL_NN: u32 = 1;
@@ -185,6 +191,15 @@ pub struct sl_paged_kv {
     pub reserved: u32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct sl_paged_tokens {
+    pub batch: u32,
+    pub tokens: u32,
+    pub row_starts: u32,
+    pub reserved: u32,
+}
+
 /// Opaque device handle.
 #[repr(C)]
 pub struct sl_hip_device {
@@ -259,6 +274,61 @@ extern "C" {
         kv_heads: u32,
         head_dim: u32,
         length: u32,
+    ) -> sl_status;
+    pub fn sl_hip_paged_append(
+        device: *mut sl_hip_device,
+        op: *const sl_op,
+        rope: *const sl_op,
+        q: *const sl_buffer_ref,
+        k: *const sl_buffer_ref,
+        v: *const sl_buffer_ref,
+        q_out: *const sl_buffer_ref,
+        tokens: *const sl_paged_tokens,
+        kv: *const sl_paged_kv,
+    ) -> sl_status;
+    pub fn sl_hip_paged_window_attention(
+        device: *mut sl_hip_device,
+        op: *const sl_op,
+        q: *const sl_buffer_ref,
+        out: *const sl_buffer_ref,
+        window: u32,
+        sinks: u32,
+        tokens: *const sl_paged_tokens,
+        kv: *const sl_paged_kv,
+    ) -> sl_status;
+    pub fn sl_hip_paged_prefix_attention(
+        device: *mut sl_hip_device,
+        op: *const sl_op,
+        q: *const sl_buffer_ref,
+        out: *const sl_buffer_ref,
+        prefix: u32,
+        tokens: *const sl_paged_tokens,
+        kv: *const sl_paged_kv,
+    ) -> sl_status;
+    pub fn sl_hip_buffer_address(
+        device: *mut sl_hip_device,
+        buffer: u32,
+        out: *mut *mut c_void,
+        elements: *mut u64,
+    ) -> sl_status;
+    pub fn sl_hip_validate_paged(
+        buffers: *const sl_buffer_desc,
+        n_buffers: usize,
+        kind: u32,
+        op: *const sl_op,
+        rope: *const sl_op,
+        q: *const sl_buffer_ref,
+        k: *const sl_buffer_ref,
+        v: *const sl_buffer_ref,
+        out: *const sl_buffer_ref,
+        window: u32,
+        sinks: u32,
+        tokens: *const sl_paged_tokens,
+        kv: *const sl_paged_kv,
+        row_starts: *const u32,
+        seq_lens: *const u32,
+        block_table: *const u32,
+        err: *mut sl_error,
     ) -> sl_status;
     pub fn sl_hip_validate_dispatch(
         buffers: *const sl_buffer_desc,

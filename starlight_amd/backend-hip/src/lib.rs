@@ -40,6 +40,36 @@ pub struct PagedKv {
     pub pages_per_seq: u32,
 }
 
+/// The new tokens of one step over a paged cache: `row_starts` u32
+/// [batch + 1], row b's tokens being `row_starts[b] .. row_starts[b + 1]`.
+#[derive(Clone, Copy, Debug)]
+pub struct PagedTokens {
+    pub batch: u32,
+    pub tokens: u32,
+    pub row_starts: BufferId,
+}
+
+impl PagedKv {
+    fn raw(&self) -> ffi::sl_paged_kv {
+        ffi::sl_paged_kv {
+            pool: self.pool.0,
+            block_table: self.block_table.0,
+            seq_lens: self.seq_lens.0,
+            layers: self.layers,
+            num_pages: self.num_pages,
+            page_size: self.page_size,
+            pages_per_seq: self.pages_per_seq,
+            reserved: 0,
+        }
+    }
+}
+
+impl PagedTokens {
+    fn raw(&self) -> ffi::sl_paged_tokens {
+        ffi::sl_paged_tokens { batch: self.batch, tokens: self.tokens, row_starts: self.row_starts.0, reserved: 0 }
+    }
+}
+
 /// The HIP device. Single owner: every method takes `&mut self`, as the
 /// trait does, and the library is not called from two threads at once.
 pub struct HipDevice {
@@ -147,19 +177,79 @@ impl HipDevice {
         kv: &PagedKv,
     ) -> Result<(), DeviceError> {
         let op = to_sl_op(op)?;
-        let raw_kv = ffi::sl_paged_kv {
-            pool: kv.pool.0,
-            block_table: kv.block_table.0,
-            seq_lens: kv.seq_lens.0,
-            layers: kv.layers,
-            num_pages: kv.num_pages,
-            page_size: kv.page_size,
-            pages_per_seq: kv.pages_per_seq,
-            reserved: 0,
-        };
+        let raw_kv = kv.raw();
         let (q, k, v, o) = (to_sl_buffer_ref(q), to_sl_buffer_ref(k_new), to_sl_buffer_ref(v_new), to_sl_buffer_ref(out));
         let status = unsafe { ffi::sl_hip_paged_attention(self.raw, &op, &q, &k, &v, &o, batch, &raw_kv) };
         self.check(status)
+    }
+
+    /// `sl_hip_paged_append`: the new tokens' keys (rotated by the Rope op
+    /// `rope`, if any) and values into layer `op`'s pages; `queries`, a pair of
+    /// source and destination, rotated the same way. No reference counterpart.
+    pub fn paged_append(
+        &mut self,
+        op: &Op,
+        rope: Option<&Op>,
+        queries: Option<(&BufferRef, &BufferRef)>,
+        k: &BufferRef,
+        v: &BufferRef,
+        tokens: &PagedTokens,
+        kv: &PagedKv,
+    ) -> Result<(), DeviceError> {
+        let op = to_sl_op(op)?;
+        let rope = rope.map(to_sl_op).transpose()?;
+        let queries = queries.map(|(q, out)| (to_sl_buffer_ref(q), to_sl_buffer_ref(out)));
+        let (k, v, tokens, kv) = (to_sl_buffer_ref(k), to_sl_buffer_ref(v), tokens.raw(), kv.raw());
+        let rope = rope.as_ref().map_or(ptr::null(), |r| r as *const _);
+        let (q, q_out) = queries.as_ref().map_or((ptr::null(), ptr::null()), |(q, o)| (q as *const _, o as *const _));
+        let status = unsafe { ffi::sl_hip_paged_append(self.raw, &op, rope, q, &k, &v, q_out, &tokens, &kv) };
+        self.check(status)
+    }
+
+    /// `sl_hip_paged_window_attention`: causal attention of the new tokens
+    /// over their rows' pages behind a sliding window with sinks (window 0: over
+    /// all positions). No reference counterpart.
+    pub fn paged_window_attention(
+        &mut self,
+        op: &Op,
+        q: &BufferRef,
+        out: &BufferRef,
+        window: u32,
+        sinks: u32,
+        tokens: &PagedTokens,
+        kv: &PagedKv,
+    ) -> Result<(), DeviceError> {
+        let op = to_sl_op(op)?;
+        let (q, o, tokens, kv) = (to_sl_buffer_ref(q), to_sl_buffer_ref(out), tokens.raw(), kv.raw());
+        let status =
+            unsafe { ffi::sl_hip_paged_window_attention(self.raw, &op, &q, &o, window, sinks, &tokens, &kv) };
+        self.check(status)
+    }
+
+    /// `sl_hip_paged_prefix_attention`: causal attention of the new tokens of
+    /// rows whose first `prefix` positions lie in the same pages. No reference
+    /// counterpart.
+    pub fn paged_prefix_attention(
+        &mut self,
+        op: &Op,
+        q: &BufferRef,
+        out: &BufferRef,
+        prefix: u32,
+        tokens: &PagedTokens,
+        kv: &PagedKv,
+    ) -> Result<(), DeviceError> {
+        let op = to_sl_op(op)?;
+        let (q, o, tokens, kv) = (to_sl_buffer_ref(q), to_sl_buffer_ref(out), tokens.raw(), kv.raw());
+        let status = unsafe { ffi::sl_hip_paged_prefix_attention(self.raw, &op, &q, &o, prefix, &tokens, &kv) };
+        self.check(status)
+    }
+
+    /// The device address of an f32 buffer and its capacity in elements,
+    /// valid until the device is dropped. No reference counterpart.
+    pub fn buffer_address(&mut self, buffer: BufferId) -> Result<(*mut std::os::raw::c_void, u64), DeviceError> {
+        let (mut address, mut elements) = (ptr::null_mut(), 0u64);
+        let status = unsafe { ffi::sl_hip_buffer_address(self.raw, buffer.0, &mut address, &mut elements) };
+        self.check(status).map(|()| (address, elements))
     }
 
     /// `sl_status` plus `sl_hip_last_error` -> `DeviceError`, variant for

@@ -40,6 +40,7 @@
 #include "arena.h"
 #include "kernels/kernels.h"
 #include "internal.h"
+#include "paged.h"
 #include "plan.h"
 #include "starlight_hip.h"
 
@@ -1622,6 +1623,165 @@ sl_status sl_hip_paged_attention(sl_hip_device* d, const sl_op* op, const sl_buf
         a, slhip::Workspace{d->workspace, d->workspace_floats}, d->stream);
     if (e == hipErrorNotSupported) return d->fail(Error::unimplemented("paged attention shape is not supported"));
     if (e != hipSuccess) return d->hip_fail(e);
+    return SL_OK;
+}
+
+}  // extern "C"
+
+namespace slhip {
+namespace {
+
+// Makes the device's GPU current for a call's launches, and the caller's again
+// after it.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(const Device* d) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != d->ordinal && hipSetDevice(d->ordinal) == hipSuccess)
+            before = now;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// Checks a call on ragged tokens, submits what is logged and launches it.
+template <typename Launch>
+sl_status paged_call(Device* d, const PagedCall& c, Launch launch) {
+    if (paged_argument_missing(c)) return d->fail(Error::execution("paged operator received a null argument"));
+    Error err;
+    PagedPlan plan;
+    try {
+        if (!check_paged_call(*d, c, &err)) return d->fail(err);
+        // (both limits are the same: every u32 buffer up to it has its host copy)
+        const Buffer& starts = d->buffers[c.tokens->row_starts];
+        const Buffer& lens = d->buffers[c.kv->seq_lens];
+        const Buffer& table = d->buffers[c.kv->block_table];
+        if (!check_paged_contents(c, {starts.mirror.data(), lens.mirror.data(), table.mirror.data()}, &plan, &err))
+            return d->fail(err);
+    } catch (...) {
+        return d->fail(Error::out_of_memory(c.kv->num_pages));
+    }
+    if (c.tokens->tokens == 0) return SL_OK;
+    const OnDevice current(d);
+    if (flush(d) != SL_OK) return d->last.status;
+    const hipError_t e = launch(plan);
+    if (e != hipSuccess) return d->hip_fail(e);
+    return SL_OK;
+}
+
+PagedTokensArgs paged_tokens_args(Device* d, const PagedCall& c, const PagedPlan& plan) {
+    PagedTokensArgs a{};
+    a.starts = static_cast<const uint32_t*>(d->buffers[c.tokens->row_starts].ptr);
+    a.lens = static_cast<const uint32_t*>(d->buffers[c.kv->seq_lens].ptr);
+    a.table = static_cast<const uint32_t*>(d->buffers[c.kv->block_table].ptr);
+    a.pool = static_cast<const float*>(d->buffers[c.kv->pool].ptr);
+    a.q = fptr(d, *c.q);
+    a.out = fptr(d, *c.out);
+    a.batch = c.tokens->batch;
+    a.tokens = c.tokens->tokens;
+    a.heads = c.op->heads;
+    a.kv_heads = c.op->kv_heads;
+    a.head_dim = c.op->head_dim;
+    a.layer = c.op->layer;
+    a.num_pages = c.kv->num_pages;
+    a.page_size = c.kv->page_size;
+    a.pages_per_seq = c.kv->pages_per_seq;
+    a.window = c.window;
+    a.sinks = c.sinks < 0x7fffffffu ? c.sinks : 0x7fffffffu;
+    a.most_keys = plan.most_keys;
+    a.scale = c.op->scale;
+    return a;
+}
+
+}  // namespace
+}  // namespace slhip
+
+extern "C" {
+
+sl_status sl_hip_paged_append(sl_hip_device* d, const sl_op* op, const sl_op* rope, const sl_buffer_ref* q,
+                              const sl_buffer_ref* k, const sl_buffer_ref* v, const sl_buffer_ref* q_out,
+                              const sl_paged_tokens* tokens, const sl_paged_kv* kv) {
+    slhip::PagedCall c;
+    c.kind = SL_PAGED_APPEND;
+    c.op = op;
+    c.rope = rope;
+    c.tokens = tokens;
+    c.kv = kv;
+    c.q = q;
+    c.k = k;
+    c.v = v;
+    c.out = q_out;
+    return slhip::paged_call(d, c, [&](const slhip::PagedPlan&) {
+        slhip::PagedAppendArgs a{};
+        a.starts = static_cast<const uint32_t*>(d->buffers[tokens->row_starts].ptr);
+        a.lens = static_cast<const uint32_t*>(d->buffers[kv->seq_lens].ptr);
+        a.table = static_cast<const uint32_t*>(d->buffers[kv->block_table].ptr);
+        if (q != nullptr) {
+            a.q = slhip::fptr(d, *q);
+            a.q_out = slhip::fptr(d, *q_out);
+        }
+        a.k = slhip::fptr(d, *k);
+        a.v = slhip::fptr(d, *v);
+        const uint64_t page = 2ull * kv->page_size * op->kv_heads * op->head_dim;
+        a.pool = static_cast<float*>(d->buffers[kv->pool].ptr) + op->layer * kv->num_pages * page;
+        a.batch = tokens->batch;
+        a.tokens = tokens->tokens;
+        a.heads = op->heads;
+        a.kv_heads = op->kv_heads;
+        a.head_dim = op->head_dim;
+        a.num_pages = kv->num_pages;
+        a.page_size = kv->page_size;
+        a.pages_per_seq = kv->pages_per_seq;
+        a.rotate = rope != nullptr;
+        a.interleaved = rope != nullptr && rope->rope_variant == SL_ROPE_GPTJ;
+        a.theta = rope != nullptr ? rope->theta : 0.f;
+        return slhip::launch_paged_append(a, d->stream);
+    });
+}
+
+sl_status sl_hip_paged_window_attention(sl_hip_device* d, const sl_op* op, const sl_buffer_ref* q,
+                                        const sl_buffer_ref* out, uint32_t window, uint32_t sinks,
+                                        const sl_paged_tokens* tokens, const sl_paged_kv* kv) {
+    slhip::PagedCall c;
+    c.kind = SL_PAGED_WINDOW;
+    c.op = op;
+    c.tokens = tokens;
+    c.kv = kv;
+    c.q = q;
+    c.out = out;
+    c.window = window;
+    c.sinks = sinks;
+    return slhip::paged_call(d, c, [&](const slhip::PagedPlan& plan) {
+        return slhip::launch_paged_window(slhip::paged_tokens_args(d, c, plan),
+                                          slhip::Workspace{d->workspace, d->workspace_floats}, d->stream);
+    });
+}
+
+sl_status sl_hip_paged_prefix_attention(sl_hip_device* d, const sl_op* op, const sl_buffer_ref* q,
+                                        const sl_buffer_ref* out, uint32_t prefix, const sl_paged_tokens* tokens,
+                                        const sl_paged_kv* kv) {
+    slhip::PagedCall c;
+    c.kind = SL_PAGED_PREFIX;
+    c.op = op;
+    c.tokens = tokens;
+    c.kv = kv;
+    c.q = q;
+    c.out = out;
+    c.prefix = prefix;
+    return slhip::paged_call(d, c, [&](const slhip::PagedPlan& plan) {
+        return slhip::launch_paged_prefix(slhip::paged_tokens_args(d, c, plan), prefix,
+                                          slhip::Workspace{d->workspace, d->workspace_floats}, d->stream);
+    });
+}
+
+sl_status sl_hip_buffer_address(sl_hip_device* d, uint32_t buffer, void** out, uint64_t* elements) {
+    if (out == nullptr) return d->fail(Error::execution("buffer address received a null argument"));
+    if (buffer >= d->buffers.size() || d->buffers[buffer].desc.kind != SL_BUFFER_F32)
+        return d->fail(Error::invalid_buffer(buffer));
+    if (slhip::flush(d) != SL_OK) return d->last.status;
+    *out = d->buffers[buffer].ptr;
+    if (elements != nullptr) *elements = d->buffers[buffer].desc.elements;
     return SL_OK;
 }
 

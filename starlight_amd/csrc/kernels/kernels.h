@@ -40,6 +40,8 @@ hipError_t load_code_gemv_dense();
 hipError_t load_code_layout();
 hipError_t load_code_matmul();
 hipError_t load_code_norm_softmax();
+hipError_t load_code_paged_append();
+hipError_t load_code_paged_attention();
 hipError_t load_code_qgemm_fp6();
 hipError_t load_code_qgemm_mfma();
 hipError_t load_code_qgemv_fused();
@@ -54,7 +56,7 @@ inline hipError_t preload_code() {
                                      load_code_qgemv_fused, load_code_qgemv_mfma, load_code_qmatmul,
                                      load_code_rope,      load_code_gemv_dense, load_code_qgemm_fp6,
                                      load_code_gemm_dense, load_code_slices, load_code_attention_bf16,
-                                     load_code_qgemv_sliced};
+                                     load_code_qgemv_sliced, load_code_paged_append, load_code_paged_attention};
     hipError_t first = hipSuccess;
     for (auto load : loads) {
         const hipError_t e = load();
@@ -206,6 +208,43 @@ hipError_t launch_paged_store(const float* state, float* pool, const uint32_t* t
                               uint64_t layers, uint64_t max_seq, uint64_t row_floats, uint64_t num_pages,
                               uint64_t page_size, uint64_t length, hipStream_t s);
 uint64_t paged_attention_workspace_floats(const PagedAttentionArgs& p);
+
+// ---- ragged new tokens over a paged cache (paged_append.hip, paged_attention.hip) ----
+// The caller has checked shapes, tables, lengths and row starts.
+struct PagedAppendArgs {
+    const uint32_t* starts;
+    const uint32_t* lens;
+    const uint32_t* table;
+    const float* q;  // null: no queries
+    const float* k;
+    const float* v;
+    float* q_out;
+    float* pool;     // the layer's first page
+    uint32_t batch, tokens, heads, kv_heads, head_dim;
+    uint32_t num_pages, page_size, pages_per_seq;
+    uint32_t rotate, interleaved;
+    float theta;
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
+
+struct PagedTokensArgs {
+    const uint32_t* starts;
+    const uint32_t* lens;
+    const uint32_t* table;
+    const float* pool;  // the whole pool
+    const float* q;
+    float* out;
+    uint32_t batch, tokens, heads, kv_heads, head_dim, layer;
+    uint32_t num_pages, page_size, pages_per_seq;
+    uint32_t window, sinks;  // window 0: none
+    // what the launch is sized for (any other lengths stay right): the most keys
+    // that one row's queries see
+    uint32_t most_keys;
+    float scale;
+};
+hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hipStream_t s);
+// Positions below `prefix` lie in the same pages for every row with tokens.
+hipError_t launch_paged_prefix(const PagedTokensArgs& a, uint32_t prefix, const Workspace& ws, hipStream_t s);
 
 // ---- dense f32 matmul (reference/matmul.rs) ----
 // out[b] = a[b or 0] x op(b[b or 0]); op = transpose when `nt`.

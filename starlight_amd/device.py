@@ -173,6 +173,13 @@ def load_library() -> ctypes.CDLL:
                                     ctypes.POINTER(ir.CBufferRef), ctypes.c_uint32, ctypes.c_void_p], ctypes.c_int),
         "sl_hip_bind_paged_state": ([P, ctypes.c_uint32, ctypes.c_void_p], ctypes.c_int),
         "sl_hip_paged_store": ([P, ctypes.c_void_p] + [ctypes.c_uint32] * 7, ctypes.c_int),
+        "sl_hip_paged_append": ([P] * 9, ctypes.c_int),
+        "sl_hip_paged_window_attention": ([P] * 4 + [ctypes.c_uint32] * 2 + [P] * 2, ctypes.c_int),
+        "sl_hip_paged_prefix_attention": ([P] * 4 + [ctypes.c_uint32] + [P] * 2, ctypes.c_int),
+        "sl_hip_buffer_address": ([P, ctypes.c_uint32, ctypes.POINTER(P), ctypes.POINTER(ctypes.c_uint64)],
+                                  ctypes.c_int),
+        "sl_hip_validate_paged": ([ctypes.POINTER(ir.CBufferDesc), ctypes.c_size_t, ctypes.c_uint32] + [P] * 6 +
+                                  [ctypes.c_uint32] * 2 + [P] * 5 + [ctypes.POINTER(ir.CError)], ctypes.c_int),
         "sl_hip_synchronize": ([P], ctypes.c_int),
         "sl_hip_last_error": ([P, ctypes.POINTER(ir.CError)], None),
         "sl_hip_bind_quantized": ([P, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
@@ -207,6 +214,20 @@ def _scalars(scalars: Sequence[int]):
     return (ctypes.c_uint32 * max(len(scalars), 1))(*[int(s) for s in scalars])
 
 
+def _ref(arg):
+    """A C reference to an Op's or BufferRef's structure; None stays null."""
+    return None if arg is None else ctypes.byref(arg.to_c())
+
+
+class _Exported:
+    """An f32 buffer under the array interface that torch reads."""
+
+    def __init__(self, device: "HipDevice", address: int, shape: Sequence[int]):
+        self.device = device  # the memory lives as long as the device is open
+        self.__cuda_array_interface__ = {"shape": tuple(int(d) for d in shape), "typestr": "<f4",
+                                         "data": (address, False), "version": 2, "strides": None}
+
+
 class HipDevice:
     """One MI355X (gfx950) device: the `sl_device::Device` contract."""
 
@@ -218,6 +239,7 @@ class HipDevice:
             raise DeviceError(STATUS_NAMES.get(status, "Execution"),
                               message=f"could not open HIP device {ordinal}")
         self._h = handle
+        self._ordinal = ordinal
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -329,6 +351,53 @@ class HipDevice:
         self._check(self._lib.sl_hip_paged_store(self._h, ctypes.addressof(paged_kv), row, state, index, max_seq,
                                                  kv_heads, head_dim, length))
 
+    def paged_append(self, op: ir.Op, rope: Optional[ir.Op], q: Optional[ir.BufferRef], k: ir.BufferRef,
+                     v: ir.BufferRef, q_out: Optional[ir.BufferRef], tokens, paged_kv) -> None:
+        """sl_hip_paged_append (starlight_amd.paged): the new keys and values
+        of `tokens` (an sl_paged_tokens structure), rotated, into the pages;
+        the queries, rotated, into q_out."""
+        self._check(self._lib.sl_hip_paged_append(self._h, _ref(op), _ref(rope), _ref(q), _ref(k), _ref(v),
+                                                  _ref(q_out), ctypes.byref(tokens), ctypes.byref(paged_kv)))
+
+    def paged_window_attention(self, op: ir.Op, q: ir.BufferRef, out: ir.BufferRef, window: int, sinks: int, tokens,
+                               paged_kv) -> None:
+        """sl_hip_paged_window_attention: attention of the new tokens over
+        their rows' pages behind a sliding window with sinks (window 0: over
+        all of them)."""
+        self._check(self._lib.sl_hip_paged_window_attention(self._h, _ref(op), _ref(q), _ref(out), window, sinks,
+                                                            ctypes.byref(tokens), ctypes.byref(paged_kv)))
+
+    def paged_prefix_attention(self, op: ir.Op, q: ir.BufferRef, out: ir.BufferRef, prefix: int, tokens,
+                               paged_kv) -> None:
+        """sl_hip_paged_prefix_attention: attention of the new tokens of rows
+        whose first `prefix` positions lie in the same pages."""
+        self._check(self._lib.sl_hip_paged_prefix_attention(self._h, _ref(op), _ref(q), _ref(out), prefix,
+                                                            ctypes.byref(tokens), ctypes.byref(paged_kv)))
+
+    # -- extension: sharing buffers with another library ------------------
+    def address(self, buffer: int) -> tuple:
+        """sl_hip_buffer_address: the device address of an f32 buffer (0 for
+        one of no elements) and its capacity in elements."""
+        out, elements = ctypes.c_void_p(), ctypes.c_uint64()
+        self._check(self._lib.sl_hip_buffer_address(self._h, buffer, ctypes.byref(out), ctypes.byref(elements)))
+        return out.value or 0, elements.value
+
+    def view_f32(self, buffer: int, shape: Sequence[int], offset: int = 0):
+        """The elements of an f32 buffer from `offset` on as a torch tensor of
+        `shape`, in place: no copy. The tensor keeps this device open (until
+        `close`); what torch's default stream does with it is ordered with
+        the device's work."""
+        import torch
+
+        address, elements = self.address(buffer)
+        n = int(np.prod(shape, dtype=np.int64))
+        if offset < 0 or n > elements - offset:
+            raise DeviceError.invalid_range(buffer, offset, n)
+        place = torch.device("cuda", self._ordinal)
+        if n == 0:
+            return torch.empty(tuple(shape), dtype=torch.float32, device=place)
+        return torch.as_tensor(_Exported(self, address + 4 * offset, shape), device=place)
+
     def synchronize(self) -> None:
         self._check(self._lib.sl_hip_synchronize(self._h))
 
@@ -370,6 +439,24 @@ class HipDevice:
         return out
 
 
+def _buffer_table(buffers: Sequence[dict]):
+    """Described buffers as a C table: {"kind": "f32"|"u32"|None, "elements":
+    n} plus, for a bound quantized payload, {"quant": (qformat, group, n, k)}."""
+    table = (ir.CBufferDesc * max(len(buffers), 1))()
+    kinds = {None: 0, "f32": 1, "u32": 2}
+    for i, b in enumerate(buffers):
+        table[i].kind = kinds[b.get("kind")]
+        table[i].elements = b.get("elements", 0)
+        if "quant" in b:
+            fmt, group, qn, qk = b["quant"]
+            table[i].quantized = 1
+            table[i].qformat = int(fmt)
+            table[i].group_size = group
+            table[i].qn = qn
+            table[i].qk = qk
+    return table
+
+
 def capabilities() -> dict:
     """DeviceCapabilities of this backend (no GPU needed)."""
     lib = load_library()
@@ -386,18 +473,7 @@ def validate_dispatch(buffers: Sequence[dict], op: ir.Op, inputs: Sequence[ir.Bu
     bound quantized payload, {"quant": (qformat, group, n, k)}. Returns the
     DeviceError dispatch would raise, or None."""
     lib = load_library()
-    table = (ir.CBufferDesc * max(len(buffers), 1))()
-    kinds = {None: 0, "f32": 1, "u32": 2}
-    for i, b in enumerate(buffers):
-        table[i].kind = kinds[b.get("kind")]
-        table[i].elements = b.get("elements", 0)
-        if "quant" in b:
-            fmt, group, qn, qk = b["quant"]
-            table[i].quantized = 1
-            table[i].qformat = int(fmt)
-            table[i].group_size = group
-            table[i].qn = qn
-            table[i].qk = qk
+    table = _buffer_table(buffers)
     if len(inputs) != len(input_values):
         return DeviceError.execution("inputs and input_values have different lengths")
     if len(outputs) != len(output_values):
@@ -409,4 +485,25 @@ def validate_dispatch(buffers: Sequence[dict], op: ir.Op, inputs: Sequence[ir.Bu
     status = lib.sl_hip_validate_dispatch(table, len(buffers), ctypes.byref(c_op), in_refs, in_vals, len(inputs),
                                           out_refs, out_vals, len(outputs), _scalars(scalars), len(scalars),
                                           ctypes.byref(err))
+    return None if status == 0 else DeviceError.from_c(err)
+
+
+PAGED_APPEND, PAGED_WINDOW, PAGED_PREFIX = 0, 1, 2
+
+
+def validate_paged(buffers: Sequence[dict], kind: int, op: ir.Op, tokens, paged_kv, row_starts, seq_lens, block_table,
+                   q: Optional[ir.BufferRef] = None, k: Optional[ir.BufferRef] = None,
+                   v: Optional[ir.BufferRef] = None, out: Optional[ir.BufferRef] = None,
+                   rope: Optional[ir.Op] = None, window: int = 0, sinks: int = 0) -> Optional[DeviceError]:
+    """The checks of the paged operator `kind` (PAGED_APPEND, PAGED_WINDOW,
+    PAGED_PREFIX; `window` is the prefix for the last) against a described
+    buffer table and host copies of its u32 buffers, without a GPU. Returns the
+    DeviceError the operator would raise, or None."""
+    lib = load_library()
+    table = _buffer_table(buffers)
+    words = [np.ascontiguousarray(a, dtype=np.uint32) for a in (row_starts, seq_lens, block_table)]
+    err = ir.CError()
+    status = lib.sl_hip_validate_paged(table, len(buffers), kind, _ref(op), _ref(rope), _ref(q), _ref(k), _ref(v),
+                                       _ref(out), window, sinks, ctypes.byref(tokens), ctypes.byref(paged_kv),
+                                       *[w.ctypes.data for w in words], ctypes.byref(err))
     return None if status == 0 else DeviceError.from_c(err)

@@ -89,6 +89,40 @@ class CPagedKv(ctypes.Structure):
                 ("pages_per_seq", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
 
 
+class CPagedTokens(ctypes.Structure):
+    """sl_paged_tokens."""
+    _fields_ = [("batch", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("row_starts", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+PAGE_NONE = 0xFFFFFFFF  # a table entry whose page has been given back
+
+
+class PagedTokens:
+    """The new tokens of one step, any number per batch row, all rows' one after
+    the other: the row starts in a device buffer, set once per step and read by
+    every layer's operators."""
+
+    def __init__(self, device, max_batch: int):
+        self.device, self.max_batch = device, max_batch
+        self.buffer = device.allocate_u32(max_batch + 1, 256)
+        self.counts: List[int] = []
+        self.c_struct = CPagedTokens(0, 0, self.buffer, 0)
+
+    def set(self, counts) -> None:
+        """Row b has counts[b] new tokens (0 for rows that sit the step out);
+        uploads the row starts."""
+        counts = [int(n) for n in counts]
+        if len(counts) > self.max_batch or any(n < 0 for n in counts):
+            raise ValueError(f"{len(counts)} rows of {counts} tokens do not fit {self.max_batch} rows")
+        starts = np.full(self.max_batch + 1, sum(counts), np.uint32)
+        starts[0] = 0
+        starts[1:len(counts) + 1] = np.cumsum(counts)
+        self.device.upload_u32(self.buffer, starts)
+        self.counts = counts
+        self.c_struct = CPagedTokens(len(counts), sum(counts), self.buffer, 0)
+
+
 class PagedKvCache:
     """A PagePool bound to device buffers: the page pool (f32), the block
     tables and the lengths (u32, uploaded by `sync`)."""
@@ -124,6 +158,29 @@ class PagedKvCache:
         if missing:
             raise ValueError(f"rows {missing} hold no sequence")
         self.device.paged_attention(op, q, k_new, v_new, out, batch, self.c_struct())
+
+    def append(self, op: ir.Op, rope: Optional[ir.Op], tokens: PagedTokens, k: ir.BufferRef, v: ir.BufferRef,
+               q: Optional[ir.BufferRef] = None, q_out: Optional[ir.BufferRef] = None) -> None:
+        """sl_hip_paged_append: stores the new tokens' keys (rotated to their
+        positions by the Rope op `rope`, if any) and values in layer
+        `op.layer`, and the rotated queries in `q_out`. Positions start at the
+        lengths last synced; reserve the rows' pages (`PagePool.reserve`) and
+        `sync` first, `set_length` after the step's last layer."""
+        self.device.paged_append(op, rope, q, k, v, q_out, tokens.c_struct, self.c_struct())
+
+    def window_attention(self, op: ir.Op, tokens: PagedTokens, q: ir.BufferRef, out: ir.BufferRef, window: int = 0,
+                         sinks: int = 0) -> None:
+        """sl_hip_paged_window_attention: causal attention of the new tokens,
+        already appended, over the last `window` positions up to their own and
+        the first `sinks`; all positions without a window."""
+        self.device.paged_window_attention(op, q, out, window, sinks, tokens.c_struct, self.c_struct())
+
+    def prefix_attention(self, op: ir.Op, tokens: PagedTokens, q: ir.BufferRef, out: ir.BufferRef,
+                         prefix: int) -> None:
+        """sl_hip_paged_prefix_attention: causal attention of the new tokens,
+        already appended, of rows that begin with the same pages for their
+        first `prefix` positions."""
+        self.device.paged_prefix_attention(op, q, out, prefix, tokens.c_struct, self.c_struct())
 
     def bind_state(self, state_buffer: int) -> None:
         """Binds a decode program's KV State buffer to this cache
