@@ -342,7 +342,8 @@ typedef struct sl_paged_tokens {
 /* The three operators below serve such a step, layer by layer: append rotates
  * and stores the new keys and values, then one of the two attentions reads them.
  * `op` is the layer's CausalAttention op (layer, heads, kv_heads, head_dim, scale;
- * head_dim a multiple of 16 up to 256, any number of query heads per KV head);
+ * head_dim a multiple of 16 up to 256, up to 1024 heads, any number of query heads
+ * per KV head);
  * q, k, v and outputs are token-major, [tokens, heads, head_dim] and [tokens,
  * kv_heads, head_dim], f32 at any offset, as projections write and read them.
  * The tables, lengths and row starts are checked on the host from the last
@@ -353,8 +354,8 @@ typedef struct sl_paged_tokens {
  * call reads the tables, lengths and row starts as they then are: they must
  * still satisfy what is said here, with the same number of tokens. seq_lens is
  * not advanced: the caller adds each row's tokens after the step. Errors beside
- * those named: UnsupportedOp for another op code; Unimplemented for a head_dim
- * or page_size not named here, buffers above 16 MiB, or a block table of more
+ * those named: UnsupportedOp for another op code; Unimplemented for a head_dim,
+ * heads or page_size not named here, buffers above 16 MiB, or a block table of more
  * than 2^31 - 1 positions; Execution for shapes, lengths, row starts, page ids
  * or aliases that do not fit; InvalidBuffer and InvalidRange as dispatch. A
  * refused call changes nothing. */

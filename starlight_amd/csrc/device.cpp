@@ -31,6 +31,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <new>
@@ -113,6 +114,10 @@ struct Device : BufferView {
             if (p.first == state) return &p.second;
         return nullptr;
     }
+    // rotation powers of the last theta and head_dim (sl_hip_paged_append)
+    RopePowers powers{};
+    float powers_theta = 0.f;
+    uint32_t powers_dim = 0;
     std::vector<uint64_t> key, prev_key;
     std::vector<GraphEntry> graphs;
     size_t last_graph = SIZE_MAX;  // entry of graphs the previous replay or capture used
@@ -1657,7 +1662,8 @@ sl_status paged_call(Device* d, const PagedCall& c, Launch launch) {
         const Buffer& starts = d->buffers[c.tokens->row_starts];
         const Buffer& lens = d->buffers[c.kv->seq_lens];
         const Buffer& table = d->buffers[c.kv->block_table];
-        if (!check_paged_contents(c, {starts.mirror.data(), lens.mirror.data(), table.mirror.data()}, &plan, &err))
+        if (!check_paged_contents(c, {starts.mirror.data(), lens.mirror.data(), table.mirror.data()}, kPagedFewRows,
+                                  &plan, &err))
             return d->fail(err);
     } catch (...) {
         return d->fail(Error::out_of_memory(c.kv->num_pages));
@@ -1690,6 +1696,10 @@ PagedTokensArgs paged_tokens_args(Device* d, const PagedCall& c, const PagedPlan
     a.window = c.window;
     a.sinks = c.sinks < 0x7fffffffu ? c.sinks : 0x7fffffffu;
     a.most_keys = plan.most_keys;
+    a.few_rows = static_cast<uint32_t>(plan.few_rows);
+    a.many_rows = static_cast<uint32_t>(plan.many_rows);
+    a.many_blocks = static_cast<uint32_t>(plan.many_blocks);
+    a.rows_with_tokens = static_cast<uint32_t>(plan.rows_with_tokens);
     a.scale = c.op->scale;
     return a;
 }
@@ -1735,8 +1745,13 @@ sl_status sl_hip_paged_append(sl_hip_device* d, const sl_op* op, const sl_op* ro
         a.pages_per_seq = kv->pages_per_seq;
         a.rotate = rope != nullptr;
         a.interleaved = rope != nullptr && rope->rope_variant == SL_ROPE_GPTJ;
-        a.theta = rope != nullptr ? rope->theta : 0.f;
-        return slhip::launch_paged_append(a, d->stream);
+        if (rope != nullptr && (d->powers_theta != rope->theta || d->powers_dim != op->head_dim)) {
+            for (uint32_t pair = 0; pair < op->head_dim / 2; ++pair)
+                d->powers.of[pair] = std::pow(static_cast<double>(rope->theta), 2.0 * pair / op->head_dim);
+            d->powers_theta = rope->theta;
+            d->powers_dim = op->head_dim;
+        }
+        return slhip::launch_paged_append(a, d->powers, d->stream);
     });
 }
 

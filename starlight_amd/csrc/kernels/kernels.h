@@ -42,6 +42,7 @@ hipError_t load_code_matmul();
 hipError_t load_code_norm_softmax();
 hipError_t load_code_paged_append();
 hipError_t load_code_paged_attention();
+hipError_t load_code_paged_tiles();
 hipError_t load_code_qgemm_fp6();
 hipError_t load_code_qgemm_mfma();
 hipError_t load_code_qgemv_fused();
@@ -56,7 +57,8 @@ inline hipError_t preload_code() {
                                      load_code_qgemv_fused, load_code_qgemv_mfma, load_code_qmatmul,
                                      load_code_rope,      load_code_gemv_dense, load_code_qgemm_fp6,
                                      load_code_gemm_dense, load_code_slices, load_code_attention_bf16,
-                                     load_code_qgemv_sliced, load_code_paged_append, load_code_paged_attention};
+                                     load_code_qgemv_sliced, load_code_paged_append, load_code_paged_attention,
+                                     load_code_paged_tiles};
     hipError_t first = hipSuccess;
     for (auto load : loads) {
         const hipError_t e = load();
@@ -223,10 +225,14 @@ struct PagedAppendArgs {
     uint32_t batch, tokens, heads, kv_heads, head_dim;
     uint32_t num_pages, page_size, pages_per_seq;
     uint32_t rotate, interleaved;
-    float theta;
 };
-hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
+// theta^(2 pair / head_dim) of each pair: a position is divided by it.
+struct RopePowers {
+    double of[128];
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, const RopePowers& powers, hipStream_t s);
 
+constexpr uint32_t kPagedFewRows = 32;
 struct PagedTokensArgs {
     const uint32_t* starts;
     const uint32_t* lens;
@@ -237,9 +243,10 @@ struct PagedTokensArgs {
     uint32_t batch, tokens, heads, kv_heads, head_dim, layer;
     uint32_t num_pages, page_size, pages_per_seq;
     uint32_t window, sinks;  // window 0: none
-    // what the launch is sized for (any other lengths stay right): the most keys
-    // that one row's queries see
-    uint32_t most_keys;
+    // what the launches are sized for (any other lengths and row starts stay right): the most
+    // keys that one row's queries see; the rows' query rows per KV head, of those with up to
+    // kPagedFewRows and of the others, and the others' blocks of 256
+    uint32_t most_keys, few_rows, many_rows, many_blocks, rows_with_tokens;
     float scale;
 };
 hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hipStream_t s);

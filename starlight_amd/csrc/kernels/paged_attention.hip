@@ -7,7 +7,7 @@
 // the keys with a running maximum.
 //
 // paged_rows serves up to 16 query rows (token, query head of one KV head) per
-// block: its four waves take 32-key tiles of their own, K and V going from the
+// block: its waves take 32-key tiles of their own, K and V going from the
 // pages straight into registers in matrix operand order, and their states are
 // combined at the end. Long key ranges are split over `splits` blocks, whose
 // partials paged_merge combines.
@@ -25,184 +25,120 @@
 // A tile whose values are not finite, or a result that is not a number, sends
 // the wave back over its tiles in plain f32 (slow_tile), where a key that a query
 // does not see contributes nothing whatever it holds.
+#include <algorithm>
+
 #include "paged_geo.h"
 
 namespace slhip {
 namespace {
 
-constexpr int kWeightTop = 14;  // weights reach fp16 as up to 2^14
-
-// One wave's tiles in plain f32: lane l works on query l % 16, in `o` (that
-// query's row in LDS) on the dims 4 i + l / 16, which no other lane touches.
-// m in units of q.k (with the factor's sign), as in the fast form.
-__device__ __forceinline__ void slow_tiles(const PagedGeo& g, const PagedKeys& keys, uint32_t b, uint32_t kvh,
-                                           uint32_t tile0, uint32_t tiles, uint32_t step, const float* qrow,
-                                           PagedMask mask, float c2, float* o, float& m, float& l) {
-    const int lane = threadIdx.x % kWave, c = lane % 16, kk = lane / 16;
-    const uint64_t row = static_cast<uint64_t>(g.kv_heads) * g.head_dim;
-    m = -INFINITY;
-    l = 0.f;
-    for (uint32_t d = kk; d < g.head_dim; d += 4) o[d] = 0.f;
-    for (uint32_t tile = tile0; tile < tiles; tile += step) {
-        float p[8];
-        float tmax = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t x = 2 * tile + i / 4;
-            p[i] = -INFINITY;
-            if (x >= keys.groups) continue;
-            if (!paged_sees(mask, g.sinks, keys.group(x) * 16 + 4 * kk + i % 4)) continue;
-            const float* k = paged_group(g, b, keys.group(x), kvh) + (4 * kk + i % 4) * row;
-            float dot = 0.f;
-#pragma unroll 1
-            for (uint32_t d = 0; d < g.head_dim; ++d) dot = fmaf(qrow[d], k[d], dot);
-            p[i] = g.scale < 0.f ? -dot : dot;
-            tmax = fmaxf(tmax, p[i]);
-        }
-        tmax = fmaxf(tmax, lane_xor16(tmax));
-        tmax = fmaxf(tmax, lane_xor32(tmax));
-        const float before = m;
-        m = fmaxf(before, tmax);
-        const float corr = before == -INFINITY ? 0.f : exp2f((before - m) * c2);
-        l *= corr;
-        if (corr != 1.f)
-            for (uint32_t d = kk; d < g.head_dim; d += 4) o[d] *= corr;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t x = 2 * tile + i / 4;
-            const bool seen = x < keys.groups && paged_sees(mask, g.sinks, keys.group(x) * 16 + 4 * kk + i % 4);
-            p[i] = seen ? exp2f((p[i] - m) * c2) : 0.f;
-            l += p[i];
-        }
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            const uint32_t x = 2 * tile + i / 16;
-            if (x >= keys.groups) break;
-            // the weight of key i for query c, from the lane that holds it
-            float w = 0.f;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const float v = __shfl(p[r], c + 16 * (i % 16 / 4));
-                w = r == i / 16 * 4 + i % 4 ? v : w;
-            }
-            if (!paged_sees(mask, g.sinks, keys.group(x) * 16 + i % 16)) continue;
-            const float* v = paged_group(g, b, keys.group(x), kvh) + paged_v_offset(g) + (i % 16) * row;
-#pragma unroll 1
-            for (uint32_t d = kk; d < g.head_dim; d += 4) o[d] = fmaf(w, v[d], o[d]);
-        }
-    }
-}
-
-// EXACT: head_dim is 64 DV; else it is smaller, a multiple of 16, and the dims past
-// it are zeros.
-template <int DV, bool EXACT>
-__global__ __launch_bounds__(256, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo g) {
+// EXACT: head_dim is 64 DV; else it is smaller, a multiple of 16, and the dims past it
+// are zeros. NW: waves (8 where LDS and registers have room for two blocks per CU's waves).
+template <int DV, bool EXACT, int NW>
+__global__ __launch_bounds__(64 * NW, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo g) {
     prefetch_kernarg<arg_bytes<PagedGeo>()>();
-    constexpr int KS = 2 * DV;  // 32-dim steps of a score
-    constexpr int DT = 4 * DV;  // 16-dim tiles of the result
-    __shared__ __align__(16) float so[4][16][64 * DV + 4];
-    __shared__ float sml[4][16][2];
+    constexpr int KS = 2 * DV;     // 32-dim steps of a score
+    constexpr int DT = 4 * DV;     // 16-dim tiles of the result
+    constexpr uint32_t M = 16;     // query rows
+    constexpr int OROW = 64 * DV + 4;
+    __shared__ __align__(16) float so[NW][M][OROW];
+    __shared__ float sml[NW][M][2];
     PagedItem it;
-    if (!paged_item(g, blockIdx.x / g.kv_heads, 16, &it)) return;  // block-uniform
+    if (!paged_item(g, g.item0 + blockIdx.x / g.kv_heads, blockIdx.y, M, &it)) return;  // block-uniform
     const int tid = threadIdx.x, lane = tid % kWave, c = lane % 16, kk = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t kvh = blockIdx.x % g.kv_heads, D = g.head_dim, G = g.group;
-    const uint32_t count = min(16u, it.n * G - it.r0);
+    const uint32_t count = min(M, it.n * G - it.r0);
     const PagedKeys keys = paged_keys(g, it, it.r0, count);
     const uint32_t tiles = (keys.groups + 1) / 2;
-    const uint32_t r = it.r0 + min(static_cast<uint32_t>(c), count - 1);
-    const uint32_t position = it.len + r / G;
-    const float* const qrow = g.q + (static_cast<uint64_t>(it.t0 + r / G) * g.heads + kvh * G + r % G) * D;
-    const PagedMask mask = paged_mask(g, position);
-    const uint64_t row = static_cast<uint64_t>(g.kv_heads) * D, voff = paged_v_offset(g);
+    const uint32_t kv_bytes = g.kv_heads * D * 4;
     const bool aligned = g.aligned != 0;
+    const uint32_t r = it.r0 + min(static_cast<uint32_t>(c), count - 1);  // query c (those past the last repeat it)
+    const auto row_of = [&](uint32_t r) -> uint64_t {
+        return static_cast<uint64_t>(it.t0 + r / G) * g.heads + kvh * G + r % G;
+    };
+    const float* const qrow = g.q + row_of(r) * D;
+    const PagedMask mask = paged_mask(g, it, it.len + r / G);
 
     float4 kx[2][KS][2], vx[8][DV];
-    // Keys past the last one re-read it (their scores are masked); a missing second
-    // group re-reads the first.
+    // A missing second group re-reads the first (its scores are masked); rows past the last
+    // key are out of the buffer's range and read as zeros.
+    const auto group_rows = [&](uint32_t tile, int s, bool values) {
+        const uint32_t grp = keys.group(min(2 * tile + s, keys.groups - 1));
+        const float* const at = paged_group(g, it.b, grp, kvh);
+        const uint32_t rows_in = min(keys.end - 16 * grp, 16u);
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(values ? at + paged_v_offset(g) : at), 0,
+                                                 (rows_in - 1) * kv_bytes + 4 * D, kBufferFlags);
+    };
     const auto load_k = [&](uint32_t tile) {
+        const uint32_t own = c * kv_bytes + 16 * kk;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const uint32_t grp = keys.group(min(2 * tile + s, keys.groups - 1));
-            const float* const at = paged_group(g, it.b, grp, kvh) + min(static_cast<uint32_t>(c), keys.end - 1 - 16 * grp) * row;
+            const auto rsrc = group_rows(tile, s, false);
 #pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    kx[s][j][h] = EXACT || 32 * j + 16 * h < D
-                                      ? *reinterpret_cast<const float4*>(at + 32 * j + 16 * h + 4 * kk)
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int j = 0; j < 2 * KS; ++j)
+                kx[s][j / 2][j % 2] = EXACT || 16u * j < D
+                                          ? __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, own + 64 * j, 0, 0))
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     };
     const auto load_v = [&](uint32_t tile) {
+        const uint32_t own = 4 * kk * kv_bytes + 16 * c;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const uint32_t grp = keys.group(min(2 * tile + s, keys.groups - 1));
-            const float* const base = paged_group(g, it.b, grp, kvh) + voff;
+            const auto rsrc = group_rows(tile, s, true);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* const at = base + min(static_cast<uint32_t>(4 * kk + i), keys.end - 1 - 16 * grp) * row;
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int J = 0; J < DV; ++J)
                     vx[4 * s + i][J] = EXACT || 64 * J + 4 * c < D
-                                           ? *reinterpret_cast<const float4*>(at + 64 * J + 4 * c)
+                                           ? __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, own + 256 * J, i * kv_bytes, 0))
                                            : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
         }
     };
-    // When a tile's rows are asked for: at head_dim 64 a tile ahead; at 128 its K and
-    // V together (registers for a tile ahead would be spilled); above, V after the
-    // scores.
+    // When a tile's rows are asked for: at head_dim 64 as soon as the registers of the tile
+    // before are free, at 128 K and V together (any earlier and they would be spilled), above V
+    // after the scores.
     constexpr bool kAhead = DV == 1, kTogether = DV <= 2;
-    const uint32_t tile0 = blockIdx.y * 4 + wave, step = 4 * gridDim.y;
+    const uint32_t tile0 = it.split * NW + wave, step = NW * it.splits;
     if (kAhead && tile0 < tiles) {
         load_k(tile0);
         load_v(tile0);
     }
     v8h qh[KS], ql[KS];
     int qe;
-    bool bad;
-    {
-        float4 qx[KS][2];
-        float most = 0.f;
-        uint32_t bits = 0;
+    bool bad = false;
+    float4 x[2 * KS];
+    load_row<2 * KS, EXACT>(qrow, aligned, D, x, [&](int j) { return 16u * j + 4 * kk; });
+    float most = 0.f;
 #pragma unroll
-        for (int j = 0; j < KS; ++j)
+    for (int j = 0; j < 2 * KS; ++j) most = max_abs(most, x[j]);
+    most = fmaxf(most, lane_xor16(most));
+    most = fmaxf(most, lane_xor32(most));
+    uint32_t flag = any_nan(x) || most == INFINITY;
+    asm volatile("" : "+v"(flag));  // (here, not at the end: it would keep the row in registers)
+    bad |= flag != 0;
+    qe = part_exponent(most);
+    // a negative factor goes into the queries, so that the largest score is the largest sum
+    const float scale = g.scale < 0.f ? -power2(qe) : power2(qe);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                qx[j][h] = EXACT || 32 * j + 16 * h < D ? load4(qrow + 32 * j + 16 * h + 4 * kk, aligned)
-                                                        : make_float4(0.f, 0.f, 0.f, 0.f);
-                most = max_abs(most, qx[j][h]);
-                // (a NaN is not seen by max_abs)
-                const float4 v = qx[j][h];
-                bits |= (v.x != v.x) | (v.y != v.y) | (v.z != v.z) | (v.w != v.w);
-            }
-        most = fmaxf(most, lane_xor16(most));
-        most = fmaxf(most, lane_xor32(most));
-        bad = bits != 0 || most == INFINITY;
-        qe = part_exponent(most);
-        // a negative factor goes into the queries, so that the largest score is the largest sum
-        const float scale = g.scale < 0.f ? -power2(qe) : power2(qe);
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                put_parts(qx[j][h].x, qx[j][h].y, scale, qh[j], ql[j], 4 * h);
-                put_parts(qx[j][h].z, qx[j][h].w, scale, qh[j], ql[j], 4 * h + 2);
-            }
-        }
+    for (int j = 0; j < KS; ++j) {
+        const Parts p = to_parts(x[2 * j], x[2 * j + 1], scale);
+        qh[j] = p.h;
+        ql[j] = p.l;
     }
     const float c2 = fabsf(g.scale) * 1.4426950408889634f;
-    // The state: query c's largest score (in units of q.k), this lane's keys' part of
-    // the sum, and O^T in units of 2^-oexp: o[4 J + e][i] is dim 64 J + 16 kk + 4 i + e.
+    // The state: query c's largest exponent, this lane's keys' part of the sum, and O^T in units
+    // of 2^-oexp: o[4 J + e][i] is dim 64 J + 16 kk + 4 i + e.
     float m = -INFINITY, l = 0.f;
     v4f o[DT];
     int oexp = 0;
     bool first = true;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
 #define SL_F16(a, b, x) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, x, 0, 0, 0)
     for (uint32_t tile = tile0; tile < tiles; tile += step) {
+        const bool more = tile + step < tiles;  // wave-uniform
         if (!kAhead) {
             load_k(tile);
             if (kTogether) load_v(tile);
@@ -220,47 +156,50 @@ __global__ __launch_bounds__(256, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo g) {
         v4f sc[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            v8h kh[KS], kl[KS];
+            Parts k[KS];
 #pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    put_parts(kx[s][j][h].x, kx[s][j][h].y, kscale, kh[j], kl[j], 4 * h);
-                    put_parts(kx[s][j][h].z, kx[s][j][h].w, kscale, kh[j], kl[j], 4 * h + 2);
-                }
+            for (int j = 0; j < KS; ++j) k[j] = to_parts(kx[s][j][0], kx[s][j][1], kscale);
             // the small products first, so that a large sum rounds once per step
             v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-                x = SL_F16(kl[j], qh[j], x);
-                x = SL_F16(kh[j], ql[j], x);
+                x = SL_F16(k[j].l, qh[j], x);
+                x = SL_F16(k[j].h, ql[j], x);
             }
 #pragma unroll
-            for (int j = 0; j < KS; ++j) x = SL_F16(kh[j], qh[j], x);
+            for (int j = 0; j < KS; ++j) x = SL_F16(k[j].h, qh[j], x);
             sc[s] = x;
         }
-        const bool more = tile + step < tiles;  // wave-uniform
         if (kAhead && more) load_k(tile + step);
         if (!kTogether) load_v(tile);
+        // Weights are 2^(x c2 - m), x in the tile's units (an exact power of two apart from q.k's):
+        // m, the largest x c2 so far once rounded, is the same number in every tile and split. A
+        // query may see none of the keys so far (m = -inf): weights and corr are 0.
         float p[8];
+        const uint32_t ga = keys.group(2 * tile), gb = keys.group(min(2 * tile + 1, keys.groups - 1));
+        const bool both = 2 * tile + 1 < keys.groups;
         float tmax = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t x = 2 * tile + i / 4;
-            const uint32_t j = keys.group(min(x, keys.groups - 1)) * 16 + 4 * kk + i % 4;
-            p[i] = x < keys.groups && paged_sees(mask, g.sinks, j) ? sc[i / 4][i % 4] : -INFINITY;
+            const uint32_t j = 16 * (i < 4 ? ga : gb) + 4 * kk + i % 4;
+            p[i] = (i < 4 || both) && paged_sees(mask, g.sinks, j) ? sc[i / 4][i % 4] : -INFINITY;
             tmax = fmaxf(tmax, p[i]);
         }
         tmax = fmaxf(tmax, lane_xor16(tmax));
         tmax = fmaxf(tmax, lane_xor32(tmax));
-        // The weights' exponents are (x - m) c2, x and m in the tile's units (an exact
-        // power of two apart from q.k's): exactly 0 for the largest, however large.
-        // A query may see none of the keys so far (m = -inf): weights and corr are 0.
-        const float unit = power2(-qe - ke);
-        const float m_new = fmaxf(m, tmax * unit);
-        const float mt = m_new * power2(qe + ke), ct = c2 * unit;
-        const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * c2);
+        const float ct = ldexpf(c2, -qe - ke);
+        const float m_new = tmax == -INFINITY ? m : fmaxf(m, tmax * ct);
+        const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
         m = m_new;
+        bad |= fabsf(m_new) > kExponentMost && m_new != -INFINITY;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = p[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(p[i], ct, -m_new));
+            sum += w;
+            p[i] = w;
+        }
+        l = l * corr + sum;
         // values
         most = 0.f;
 #pragma unroll
@@ -272,46 +211,34 @@ __global__ __launch_bounds__(256, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo g) {
         const int need = part_exponent(most);
         const int ve = first ? need : min(need, oexp - kWeightTop);
         // O's unit: the weights' 2^14 times the values' scale, lowered when larger values come
-        const float turn = first ? 0.f : corr * power2(ve + kWeightTop - oexp);
+        const float turn = first ? 0.f : power2(ve + kWeightTop - oexp);
         first = false;
         oexp = ve + kWeightTop;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] *= turn;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float w = p[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((p[i] - mt) * ct);
-            sum += w;
-            p[i] = w;
-        }
-        l = l * corr + sum;
-        v8h ph, pl;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) put_parts(p[i], p[i + 1], power2(kWeightTop), ph, pl, i);
+        #pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= corr * turn;
+        const Parts w = to_parts(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], power2(kWeightTop));
         const float vscale = power2(ve);
 #pragma unroll
         for (int J = 0; J < DV; ++J)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v8h vh, vl;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                    put_parts(reinterpret_cast<const float*>(&vx[i][J])[e],
-                              reinterpret_cast<const float*>(&vx[i + 1][J])[e], vscale, vh, vl, i);
+                const auto at = [&](int i) { return reinterpret_cast<const float*>(&vx[i][J])[e]; };
+                const Parts v = to_parts(at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), vscale);
                 v4f x = o[4 * J + e];
-                x = SL_F16(vl, ph, x);
-                x = SL_F16(vh, pl, x);
-                o[4 * J + e] = SL_F16(vh, ph, x);
+                x = SL_F16(v.l, w.h, x);
+                x = SL_F16(v.h, w.l, x);
+                o[4 * J + e] = SL_F16(v.h, w.h, x);
             }
         if (kAhead && more) load_v(tile + step);
     }
 #undef SL_F16
     const float back = power2(-oexp);
-    float check = l;
+    float check = 0.f;
+    check += l;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-        o[t] *= back;
-        check += (o[t][0] + o[t][1]) + (o[t][2] + o[t][3]);
+    for (int d = 0; d < DT; ++d) {
+        o[d] *= back;
+        check += (o[d][0] + o[d][1]) + (o[d][2] + o[d][3]);
     }
     // (an infinite check of finite values, near f32's end, only costs time)
     bad |= !(fabsf(check) < INFINITY);
@@ -333,56 +260,84 @@ __global__ __launch_bounds__(256, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo g) {
     }
     __syncthreads();
     const uint32_t d4 = D / 4;
-    for (uint32_t i = tid; i < count * d4; i += 256) {
+    for (uint32_t i = tid; i < count * d4; i += 64 * NW) {
         const uint32_t x = i / d4, d = 4 * (i % d4);
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w][x][0]);
+        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sml[w][x][0]);
         float sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float mw = sml[w][x][0];
             // (an empty state weighs nothing; a NaN maximum keeps its sum's NaN)
-            const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - mm) * c2);
+            const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
             sum = fmaf(sml[w][x][1], f, sum);
             if (f != 0.f) fma4(acc, f, *reinterpret_cast<const float4*>(&so[w][x][d]));
         }
-        const uint32_t rr = it.r0 + x;
-        const uint64_t at = static_cast<uint64_t>(it.t0 + rr / G) * g.heads + kvh * G + rr % G;
+        const uint64_t at = row_of(it.r0 + x);
         if (g.slots == 1) {
             store4(g.out + at * D + d, scaled4(acc, 1.0f / sum), aligned);
         } else {
-            const uint64_t slot = at * g.slots + g.slot0 + blockIdx.y;
+            const uint64_t slot = at * g.slots + it.slot;
             *reinterpret_cast<float4*>(g.part + slot * D + d) = acc;
             if (d == 0) g.ml[slot] = make_float2(mm, sum);
         }
     }
 }
 
-// Combines the partials of each query row: thread per float4 of the result.
+// Combines the partials of each query row. A block has up to 16 query rows, a
+// thread one float4 of one of them. The (m, sum) pairs of its rows come
+// to LDS while the first partials are on their way; the weights 2^(m - max) / sum
+// are worked out once per row and partial.
+constexpr uint32_t kMergeRows = 16, kMergeSlots = 128;
+
 __global__ __launch_bounds__(256) void paged_merge(PagedGeo g) {
     prefetch_kernarg<arg_bytes<PagedGeo>()>();
-    const uint32_t d4 = g.head_dim / 4;
-    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= static_cast<uint64_t>(g.tokens) * g.heads * d4) return;
-    const uint64_t at = i / d4;
-    const uint32_t d = 4 * static_cast<uint32_t>(i % d4);
-    const float c2 = fabsf(g.scale) * 1.4426950408889634f;
-    const float2* const ml = g.ml + at * g.slots;
-    const float* const part = g.part + at * g.slots * g.head_dim + d;
+    constexpr int U = 8;  // partials in flight
+    __shared__ float2 ml[kMergeRows][kMergeSlots];
+    const uint32_t tid = threadIdx.x, d4 = g.head_dim / 4, S = g.slots;
+    const uint32_t rows = min(256 / d4, kMergeRows);
+    const uint64_t all = static_cast<uint64_t>(g.tokens) * g.heads, row0 = static_cast<uint64_t>(blockIdx.x) * rows;
+    const uint32_t here = static_cast<uint32_t>(min(all - row0, static_cast<uint64_t>(rows)));
+    const uint32_t x = min(tid / d4, here - 1), c = tid % d4;
+    const uint64_t at = row0 + x;
+    const float* const part = g.part + at * S * g.head_dim + 4 * c;
+    float4 v[U];
+    const auto load = [&](uint32_t s0) {  // (past the last they re-read it, with weight 0)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] = *reinterpret_cast<const float4*>(part + static_cast<uint64_t>(min(s0 + u, S - 1)) * g.head_dim);
+    };
+    for (uint32_t i = tid; i < here * S; i += 256) ml[i / S][i % S] = g.ml[row0 * S + i];
+    load(0);
+    __syncthreads();
     float mm = -INFINITY;
-    for (uint32_t s = 0; s < g.slots; ++s) mm = fmaxf(mm, ml[s].x);
+    for (uint32_t s = 0; s < S; ++s) mm = fmaxf(mm, ml[x][s].x);
+    __syncthreads();
+    // each of a row's threads its share of the weights (a NaN maximum keeps its sum's NaN)
+    if (tid / d4 < here)
+        for (uint32_t s = c; s < S; s += d4) {
+            const float2 p = ml[x][s];
+            const float f = p.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p.x - mm);
+            ml[x][s] = make_float2(f, p.y * f);
+        }
+    __syncthreads();
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s = 0; s < g.slots; ++s) {
-        const float2 x = ml[s];
-        const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - mm) * c2);
-        l = fmaf(x.y, f, l);
-        if (f == 0.f) continue;
-        fma4(o, f, *reinterpret_cast<const float4*>(part + static_cast<uint64_t>(s) * g.head_dim));
+    for (uint32_t s0 = 0; s0 < S; s0 += U) {
+        if (s0 != 0) load(s0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u >= S) continue;
+            const float2 p = ml[x][s0 + u];
+            l += p.y;
+            // (an empty partial's values are zeros)
+            fma4(o, p.x, v[u]);
+        }
     }
-    store4(g.out + at * g.head_dim + d, scaled4(o, 1.0f / l), g.aligned != 0);
+    if (tid / d4 < here)
+        store4(g.out + at * g.head_dim + 4 * c, scaled4(o, 1.0f / l), g.aligned != 0);
 }
 
 }  // namespace
@@ -405,12 +360,11 @@ PagedGeo paged_geometry(const PagedTokensArgs& a) {
     g.group = a.heads / a.kv_heads;
     g.head_dim = a.head_dim;
     g.page16 = a.page_size / 16;
+    g.page_shift = (g.page16 & (g.page16 - 1)) == 0 ? static_cast<uint32_t>(__builtin_ctz(g.page16)) : 32;
     g.pages_per_seq = a.pages_per_seq;
     g.num_pages = a.num_pages;
     g.window = a.window == 0 ? 0xffffffffu : a.window;
     g.sinks = a.window == 0 ? 0 : a.sinks;
-    g.kbegin = 0;
-    g.kend = 0xffffffffu;
     g.splits = g.slots = 1;
     g.aligned = aligned16(a.q) && aligned16(a.out);
     g.rows_upto = 0xffffffffu;
@@ -418,29 +372,39 @@ PagedGeo paged_geometry(const PagedTokensArgs& a) {
     return g;
 }
 
-// One launch over the geometry's keys, `splits` blocks per item.
-hipError_t launch_rows(const PagedGeo& g, hipStream_t s) {
-    const uint64_t rows = static_cast<uint64_t>(g.tokens) * g.group;
-    const uint64_t items = g.shared ? (rows + 15) / 16 : rows / 16 + g.batch;
-    const dim3 grid(static_cast<unsigned>(items * g.kv_heads), g.splits);
-    const uint32_t dv = (g.head_dim + 63) / 64;
+constexpr uint32_t kBlockRows = 16;  // query rows of a paged_rows block
+
+// Items of a launch with `per` query rows each: the shared ones, and the rows' own.
+uint64_t shared_items(const PagedGeo& g, uint64_t per) {
+    return (static_cast<uint64_t>(g.tokens) * g.group + per - 1) / per;
+}
+uint64_t own_items(const PagedGeo& g, uint64_t per) {
+    return static_cast<uint64_t>(g.tokens) * g.group / per + g.batch;
+}
+
+hipError_t launch_rows(const PagedGeo& g, uint64_t items, hipStream_t s) {
+    const uint32_t splits = std::max(g.item0 < g.shared_items ? g.shared_splits : 0, g.splits);
+    const dim3 grid(static_cast<unsigned>(items * g.kv_heads), splits);
     const bool exact = g.head_dim % 64 == 0;
-#define SL_ROWS(DV)                                           \
-    if (exact) paged_rows<DV, true><<<grid, 256, 0, s>>>(g);  \
-    else paged_rows<DV, false><<<grid, 256, 0, s>>>(g)
-    switch (dv) {
-        case 1: SL_ROWS(1); break;
-        case 2: SL_ROWS(2); break;
-        case 3: SL_ROWS(3); break;
-        default: SL_ROWS(4); break;
+#define SL_ROWS(DV, NW)                                               \
+    do {                                                              \
+        if (exact) paged_rows<DV, true, NW><<<grid, 64 * NW, 0, s>>>(g); \
+        else paged_rows<DV, false, NW><<<grid, 64 * NW, 0, s>>>(g);      \
+    } while (0)
+    switch ((g.head_dim + 63) / 64) {
+        case 1: SL_ROWS(1, 8); break;
+        case 2: SL_ROWS(2, 8); break;
+        case 3: SL_ROWS(3, 4); break;
+        default: SL_ROWS(4, 4); break;
     }
 #undef SL_ROWS
     return hipGetLastError();
 }
 
 hipError_t launch_merge(const PagedGeo& g, hipStream_t s) {
-    const uint64_t n = static_cast<uint64_t>(g.tokens) * g.heads * (g.head_dim / 4);
-    paged_merge<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(g);
+    const uint64_t rows = std::min<uint64_t>(1024 / g.head_dim, kMergeRows);
+    const uint64_t blocks = (static_cast<uint64_t>(g.tokens) * g.heads + rows - 1) / rows;
+    paged_merge<<<static_cast<unsigned>(blocks), 256, 0, s>>>(g);
     return hipGetLastError();
 }
 
@@ -455,24 +419,59 @@ bool place_partials(PagedGeo* g, uint32_t slots, const Workspace& ws) {
     return true;
 }
 
-// Key splits for `items` blocks per KV head that read up to `keys` keys each: until
-// about two blocks per CU run, each wave having a tile of 32 keys.
-uint32_t splits_for(uint64_t items, uint64_t kv_heads, uint64_t keys) {
-    const uint64_t blocks = items * kv_heads, most = (keys + 127) / 128;
-    uint64_t n = blocks ? (2 * compute_units() + blocks - 1) / blocks : 1;
-    n = n < most ? n : most;
-    return static_cast<uint32_t>(n < 1 ? 1 : n > 64 ? 64 : n);
+// Key splits for `blocks` blocks of equal work, one per CU at a time, whose keys take `steps`
+// steps (256 keys of paged_rows, 64 of paged_tiles): a round of blocks costs its steps and
+// `fixed` more, partials a step or two. (1 for a batch that fills the chip by itself; 2 for
+// blocks that would leave a second round half empty.)
+uint32_t splits_for(uint64_t blocks, uint64_t steps, double fixed) {
+    const uint64_t cus = compute_units();
+    if (blocks == 0) return 1;
+    uint32_t best = 1;
+    double least = 0.0;
+    for (uint32_t n = 1; n <= kMergeSlots / 2 && n <= steps; ++n) {
+        const double rounds = static_cast<double>((blocks * n + cus - 1) / cus);
+        const double cost = rounds * (static_cast<double>(steps) / n + fixed) + (n > 1 ? 1.5 : 0.0);
+        if (n == 1 || cost < least) {
+            least = cost;
+            best = n;
+        }
+    }
+    return best;
 }
+constexpr double kRowsFixed = 0.5, kTilesFixed = 4.0;  // measured: about 4 us and 20 us
+
+// Bytes of K and V that sharing has to save, and query rows up to which the shared part is
+// paged_rows' (8B shapes, 16 rows over a prefix of 2,000: 27.9 us, with paged_tiles 42.0; 34 tokens
+// of 8 rows over 4,096: 54.1, with paged_tiles 52.4; 64 over 16,384: 262, with paged_tiles 143).
+constexpr uint64_t kSharingPays = 24ull << 20;
+constexpr uint64_t kSharedFewRows = 64;
 
 }  // namespace
 
 hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hipStream_t s) {
     if (a.tokens == 0) return hipSuccess;
     PagedGeo g = paged_geometry(a);
-    const uint64_t rows = static_cast<uint64_t>(g.tokens) * g.group;
-    const uint32_t splits = splits_for(rows / 16 + g.batch, g.kv_heads, a.most_keys);
+    // rows of a sequence's tokens go to paged_rows up to kPagedFewRows query rows, above to
+    // paged_tiles: which launches there are, and their splits, follow the row starts of this call;
+    // each launch takes the rows that are its own when it runs
+    const bool tiles = a.many_rows != 0 && g.head_dim <= 128, some = !tiles || a.few_rows != 0;
+    const uint64_t few = a.few_rows + (tiles ? 0 : a.many_rows);
+    uint32_t splits = 1;
+    if (some) splits = splits_for((few + kBlockRows - 1) / kBlockRows * g.kv_heads, (a.most_keys + 255) / 256, kRowsFixed);
+    if (tiles)
+        splits = splits_for(static_cast<uint64_t>(a.many_blocks) * g.kv_heads, (a.most_keys + 63) / 64, kTilesFixed);
     if (splits > 1 && place_partials(&g, splits, ws)) g.splits = splits;
-    hipError_t e = launch_rows(g, s);
+    hipError_t e = hipSuccess;
+    if (some) {
+        PagedGeo x = g;
+        if (tiles) x.rows_upto = kPagedFewRows;
+        e = launch_rows(x, own_items(g, kBlockRows), s);
+    }
+    if (e == hipSuccess && tiles) {
+        PagedGeo x = g;
+        if (some) x.rows_over = kPagedFewRows;
+        e = launch_paged_tiles(x, own_items(g, kTileRows), s);
+    }
     if (e == hipSuccess && g.slots > 1) e = launch_merge(g, s);
     return e;
 }
@@ -481,18 +480,28 @@ hipError_t launch_paged_prefix(const PagedTokensArgs& a, uint32_t prefix, const 
     if (a.tokens == 0) return hipSuccess;
     PagedGeo g = paged_geometry(a);
     const uint64_t rows = static_cast<uint64_t>(g.tokens) * g.group;
-    const uint32_t first = splits_for((rows + 15) / 16, g.kv_heads, prefix);
-    const uint32_t second = splits_for(rows / 16 + g.batch, g.kv_heads, a.most_keys - prefix);
-    if (prefix == 0 || !place_partials(&g, first + second, ws)) return launch_paged_window(a, ws, s);
-    PagedGeo own = g;
-    g.shared = 1;
-    g.kend = prefix;
-    g.splits = first;
-    own.kbegin = prefix;
-    own.splits = second;
-    own.slot0 = first;
-    hipError_t e = launch_rows(g, s);
-    if (e == hipSuccess) e = launch_rows(own, s);
+    // Sharing costs partials of every query row: it does not pay where the rows read little more
+    // on their own (what they share then comes from the caches).
+    const uint64_t saved = static_cast<uint64_t>(prefix) * (a.rows_with_tokens - 1) * g.kv_heads * g.head_dim * 8;
+    if (saved < kSharingPays) return launch_paged_window(a, ws, s);
+    const bool tiles = g.head_dim <= 128 && rows > kSharedFewRows;
+    const uint64_t shared = shared_items(g, tiles ? kTileRows : kBlockRows);
+    const uint64_t few = a.few_rows + a.many_rows;
+    g.shared_splits = tiles ? splits_for(shared * g.kv_heads, (prefix + 63) / 64, kTilesFixed)
+                            : splits_for(shared * g.kv_heads, (prefix + 255) / 256, kRowsFixed);
+    g.splits = splits_for((few + kBlockRows - 1) / kBlockRows * g.kv_heads, (a.most_keys - prefix + 255) / 256, kRowsFixed);
+    if (!place_partials(&g, g.shared_splits + g.splits, ws)) return launch_paged_window(a, ws, s);
+    g.prefix = prefix;
+    g.shared_items = static_cast<uint32_t>(shared);
+    hipError_t e = hipSuccess;
+    if (tiles) {
+        e = launch_paged_tiles(g, shared, s);
+        // (the rows' own items are counted in paged_rows' measure)
+        g.item0 = g.shared_items;
+        if (e == hipSuccess) e = launch_rows(g, own_items(g, kBlockRows), s);
+    } else {
+        e = launch_rows(g, shared + own_items(g, kBlockRows), s);  // both kinds beside one another
+    }
     if (e == hipSuccess) e = launch_merge(g, s);
     return e;
 }

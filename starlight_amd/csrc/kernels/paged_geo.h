@@ -7,7 +7,6 @@
 #include "kernels.h"
 
 namespace slhip {
-namespace {
 
 // The new tokens of all rows lie one after the other: q and out are
 // [tokens, heads, head_dim], row b's tokens are starts[b] .. starts[b + 1],
@@ -22,30 +21,48 @@ struct PagedGeo {
     const float* q;
     float* out;
     float* part;   // partial results [token][head][slot][head_dim], not yet divided by their sums
-    float2* ml;    // [token][head][slot]: the partial's largest score and sum of weights
+    float2* ml;    // [token][head][slot]: the partial's largest exponent and sum of weights
     uint32_t batch, tokens, heads, kv_heads, group, head_dim;
-    uint32_t page16, pages_per_seq, num_pages;  // page16: 16-position groups per page
+    uint32_t page16, pages_per_seq, num_pages;  // page16: 16-position groups per page,
+    uint32_t page_shift;                        // its logarithm, or 32 where it is no power of two
     uint32_t window, sinks;                     // window 0xffffffff: none
-    uint32_t kbegin, kend;                      // only keys kbegin <= j < kend
-    uint32_t splits, slots, slot0;              // key splits of this launch; slots per query row, the launch's first
+    // Items of a launch: first shared_items of them (from item0 on) are all tokens' queries over
+    // the positions below `prefix`, which lie in the same pages for every row; the others are each
+    // row's queries over its positions from `prefix` on.
+    uint32_t prefix, shared_items, item0;
+    uint32_t shared_splits, splits, slots;  // key splits of the two kinds; partials per query row, the shared first
     uint32_t aligned;                           // q and out are 16-byte aligned
-    uint32_t shared;                            // all tokens are one row's (the shared prefix)
     uint32_t rows_over, rows_upto;              // rows with rows_over < query rows <= rows_upto, the others exit
     float scale;
 };
 
-// One block's row and its first query row.
+// paged_tiles.hip: the form for many query rows per KV head, kTileRows per block, head_dim up to
+// 128. One launch over `items` items.
+constexpr uint32_t kTileRows = 256;
+hipError_t launch_paged_tiles(const PagedGeo& g, uint64_t items, hipStream_t s);
+
+namespace {
+
+// One block's row, its first query row, and which keys it takes: begin <= j < end, split
+// number `split` of `splits`, whose partial is `slot`.
 struct PagedItem {
     uint32_t b, len, n, t0, r0;
+    uint32_t begin, end, splits, split, slot;
 };
 
 // Item x of a grid with M query rows per item. Row b has the items from
-// starts[b] * group / M + b on: at least as many as its query rows need, and
-// found from starts alone. Every wave of a block comes to the same answer.
-// False: the item has no query rows.
-__device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t x, uint32_t M, PagedItem* it) {
+// starts[b] * group / M + b on (after the shared ones): at least as many as its query rows
+// need, and found from starts alone. Every wave of a block comes to the same answer. False:
+// nothing to do.
+__device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t item, uint32_t split, uint32_t M, PagedItem* it) {
     const uint32_t lane = threadIdx.x % kWave;
-    if (g.shared) {
+    it->split = split;
+    if (item < g.shared_items) {
+        if (split >= g.shared_splits) return false;
+        it->begin = 0;
+        it->end = g.prefix;
+        it->splits = g.shared_splits;
+        it->slot = split;
         // (the first row that has a token: its table names the shared pages)
         uint32_t row = 0;
         for (uint32_t b0 = 0; b0 < g.batch; b0 += kWave) {
@@ -57,12 +74,18 @@ __device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t x, uint32
             }
         }
         it->b = __builtin_amdgcn_readfirstlane(row);
-        it->len = g.kend;
+        it->len = g.prefix;
         it->n = g.tokens;
         it->t0 = 0;
-        it->r0 = x * M;
+        it->r0 = item * M;
         return it->r0 < it->n * g.group;
     }
+    if (split >= g.splits) return false;
+    const uint32_t x = item - g.shared_items;
+    it->begin = g.prefix;
+    it->end = 0xffffffffu;
+    it->splits = g.splits;
+    it->slot = (g.prefix != 0 ? g.shared_splits : 0) + split;
     uint32_t row = 0, start = 0, next = 0, len = 0, base = 0;
     for (uint32_t b0 = 0; b0 < g.batch; b0 += kWave) {
         const uint32_t b = min(b0 + lane, g.batch - 1);
@@ -106,8 +129,8 @@ struct PagedKeys {
 __device__ __forceinline__ PagedKeys paged_keys(const PagedGeo& g, const PagedItem& it, uint32_t r0, uint32_t count) {
     const uint32_t lo = it.len + r0 / g.group, hi = it.len + (r0 + count - 1) / g.group;
     PagedKeys k;
-    k.end = min(hi + 1, g.kend);
-    const uint32_t first = max(lo >= g.window ? lo - g.window + 1 : 0, g.kbegin);
+    k.end = min(hi + 1, it.end);
+    const uint32_t first = max(lo >= g.window ? lo - g.window + 1 : 0, it.begin);
     k.first_group = first / 16;
     k.sink_groups = min((g.sinks + 15) / 16, k.first_group);
     const uint32_t last = (k.end + 15) / 16;
@@ -119,22 +142,50 @@ __device__ __forceinline__ PagedKeys paged_keys(const PagedGeo& g, const PagedIt
 struct PagedMask {
     uint32_t low, end;
 };
-__device__ __forceinline__ PagedMask paged_mask(const PagedGeo& g, uint32_t position) {
-    return {max(position >= g.window ? position - g.window + 1 : 0, g.kbegin), min(position + 1, g.kend)};
+__device__ __forceinline__ PagedMask paged_mask(const PagedGeo& g, const PagedItem& it, uint32_t position) {
+    return {max(position >= g.window ? position - g.window + 1 : 0, it.begin), min(position + 1, it.end)};
 }
 __device__ __forceinline__ bool paged_sees(const PagedMask& m, uint32_t sinks, uint32_t j) {
     return j < m.end && (j >= m.low || j < sinks);
 }
 
+// The kernel's geometry, its only argument, read again: what only the end of a
+// kernel needs would otherwise hold scalar registers through its loop.
+__device__ __forceinline__ PagedGeo geometry_again() {
+    typedef __attribute__((address_space(4))) const uint64_t word;
+    word* p = (word*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    struct Words {
+        uint64_t w[sizeof(PagedGeo) / 8];
+    } words;
+    static_assert(sizeof(PagedGeo) % 8 == 0, "whole words");
+#pragma unroll
+    for (size_t i = 0; i < sizeof(PagedGeo) / 8; ++i) words.w[i] = p[i];
+    return __builtin_bit_cast(PagedGeo, words);
+}
+
+// Word i of a table that no kernel writes, the same for the whole wave: a scalar load.
+__device__ __forceinline__ uint32_t uniform_word(const uint32_t* table, uint64_t i) {
+    typedef __attribute__((address_space(4))) const uint32_t word;
+    const uint64_t at = reinterpret_cast<uint64_t>(table + i);
+    // (the builtin returns a signed value: widened as it is, it would fill the upper half)
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at)),
+                   hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+    return *reinterpret_cast<word*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // First element of the K rows of group `grp` (positions 16 grp ..) of row b for
-// KV head kvh; a position's row is kv_heads * head_dim further, V one page half.
+// KV head kvh (all uniform over the wave); a position's row is kv_heads * head_dim further, V one page half.
 __device__ __forceinline__ const float* paged_group(const PagedGeo& g, uint32_t b, uint32_t grp, uint32_t kvh) {
-    const uint32_t pi = min(grp / g.page16, g.pages_per_seq - 1);
-    const uint32_t page = min(g.table[static_cast<uint64_t>(b) * g.pages_per_seq + pi], g.num_pages - 1);
+    const uint32_t whole = g.page_shift < 32 ? grp >> g.page_shift : grp / g.page16;
+    const uint32_t pi = min(whole, g.pages_per_seq - 1);
+    const uint32_t page = min(uniform_word(g.table, static_cast<uint64_t>(b) * g.pages_per_seq + pi), g.num_pages - 1);
     const uint64_t row = static_cast<uint64_t>(g.kv_heads) * g.head_dim;
-    return g.pool + (static_cast<uint64_t>(page) * 2 * g.page16 + grp % g.page16) * 16 * row +
+    return g.pool + (static_cast<uint64_t>(page) * 2 * g.page16 + (grp - whole * g.page16)) * 16 * row +
            static_cast<uint64_t>(kvh) * g.head_dim;
 }
+// Of a buffer resource: 32-bit words, no swizzle.
+constexpr int kBufferFlags = 0x00027000;
 __device__ __forceinline__ uint64_t paged_v_offset(const PagedGeo& g) {
     return static_cast<uint64_t>(g.page16) * 16 * g.kv_heads * g.head_dim;
 }
@@ -151,6 +202,7 @@ __device__ __forceinline__ uint64_t paged_v_offset(const PagedGeo& g) {
 // matrix instructions do.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kPartTop = 14;  // the largest value's exponent after scaling
@@ -164,13 +216,30 @@ __device__ __forceinline__ int part_exponent(float most) {
 __device__ __forceinline__ float power2(int e) {  // 2^e, 0 and infinity outside f32's normal numbers
     return e < -126 ? 0.f : e > 127 ? INFINITY : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
-__device__ __forceinline__ void put_parts(float x, float y, float scale, v8h& h, v8h& l, int i) {
-    const float a = x * scale, b = y * scale;
-    const _Float16 ha = static_cast<_Float16>(a), hb = static_cast<_Float16>(b);
-    h[i] = ha;
-    h[i + 1] = hb;
-    l[i] = static_cast<_Float16>(a - static_cast<float>(ha));
-    l[i + 1] = static_cast<_Float16>(b - static_cast<float>(hb));
+// Both parts of eight values: x scale - h is exact before it is rounded. (Packed
+// conversions and mixed multiply-adds; one multiply-add per part that rounds to fp16
+// itself, a mix instruction of half the rate, measured 2-3% slower throughout.)
+struct Parts {
+    v8h h, l;
+};
+__device__ __forceinline__ Parts to_parts(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                          float scale) {
+    const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+    Parts p;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const v2h hp = __builtin_convertvector(v2f{x[i] * scale, x[i + 1] * scale}, v2h);
+        const v2h lp = __builtin_convertvector(
+            v2f{fmaf(x[i], scale, -static_cast<float>(hp[0])), fmaf(x[i + 1], scale, -static_cast<float>(hp[1]))}, v2h);
+        p.h[i] = hp[0];
+        p.h[i + 1] = hp[1];
+        p.l[i] = lp[0];
+        p.l[i + 1] = lp[1];
+    }
+    return p;
+}
+__device__ __forceinline__ Parts to_parts(float4 a, float4 b, float scale) {
+    return to_parts(a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, scale);
 }
 __device__ __forceinline__ float max_abs(float m, float4 v) {
     m = fmaxf(fmaxf(m, fabsf(v.x)), fabsf(v.y));
@@ -188,6 +257,28 @@ __device__ __forceinline__ float4 load4(const float* p, bool aligned) {
     if (aligned) return *reinterpret_cast<const float4*>(p);
     return make_float4(p[0], p[1], p[2], p[3]);
 }
+// N float4 of a row, `at(i)` elements in, zeros from element `dims` on: all loads
+// together, under one branch (a branch each would wait for each).
+template <int N, bool EXACT, typename At>
+__device__ __forceinline__ void load_row(const float* row, bool aligned, uint32_t dims, float4 (&x)[N], At at) {
+    if (aligned) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x[i] = EXACT || at(i) < dims ? *reinterpret_cast<const float4*>(row + at(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x[i] = EXACT || at(i) < dims ? load4(row + at(i), false) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+}
+// Whether a value of x is a NaN (max_abs passes over them).
+template <int N>
+__device__ __forceinline__ bool any_nan(const float4 (&x)[N]) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) nan |= (x[i].x != x[i].x) | (x[i].y != x[i].y) | (x[i].z != x[i].z) | (x[i].w != x[i].w);
+    return nan;
+}
 __device__ __forceinline__ void store4(float* p, float4 v, bool aligned) {
     if (aligned) {
         *reinterpret_cast<float4*>(p) = v;
@@ -196,6 +287,73 @@ __device__ __forceinline__ void store4(float* p, float4 v, bool aligned) {
         p[1] = v.y;
         p[2] = v.z;
         p[3] = v.w;
+    }
+}
+
+// Exponents beyond this have no fraction worth the name, and the largest one's rounding
+// error would reach the weights' range: left to the plain form.
+constexpr float kExponentMost = 134217728.f;
+
+constexpr int kWeightTop = 14;  // weights reach fp16 as up to 2^14
+
+// One wave's tiles in plain f32: lane l works on query l % 16, in `o` (that
+// query's row in LDS) on the dims 4 i + l / 16, which no other lane touches.
+// m in units of the weights' exponents, as in the fast form.
+__device__ __forceinline__ void slow_tiles(const PagedGeo& g, const PagedKeys& keys, uint32_t b, uint32_t kvh,
+                                           uint32_t tile0, uint32_t tiles, uint32_t step, const float* qrow,
+                                           PagedMask mask, float c2, float* o, float& m, float& l) {
+    const int lane = threadIdx.x % kWave, c = lane % 16, kk = lane / 16;
+    const uint64_t row = static_cast<uint64_t>(g.kv_heads) * g.head_dim;
+    m = -INFINITY;
+    l = 0.f;
+    for (uint32_t d = kk; d < g.head_dim; d += 4) o[d] = 0.f;
+    for (uint32_t tile = tile0; tile < tiles; tile += step) {
+        float p[8];
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t x = 2 * tile + i / 4;
+            p[i] = -INFINITY;
+            if (x >= keys.groups) continue;
+            if (!paged_sees(mask, g.sinks, keys.group(x) * 16 + 4 * kk + i % 4)) continue;
+            const float* k = paged_group(g, b, keys.group(x), kvh) + (4 * kk + i % 4) * row;
+            float dot = 0.f;
+#pragma unroll 1
+            for (uint32_t d = 0; d < g.head_dim; ++d) dot = fmaf(qrow[d], k[d], dot);
+            p[i] = (g.scale < 0.f ? -dot : dot) * c2;
+            tmax = fmaxf(tmax, p[i]);
+        }
+        tmax = fmaxf(tmax, lane_xor16(tmax));
+        tmax = fmaxf(tmax, lane_xor32(tmax));
+        const float before = m;
+        m = fmaxf(before, tmax);
+        const float corr = before == -INFINITY ? 0.f : exp2f(before - m);
+        l *= corr;
+        if (corr != 1.f)
+            for (uint32_t d = kk; d < g.head_dim; d += 4) o[d] *= corr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t x = 2 * tile + i / 4;
+            const bool seen = x < keys.groups && paged_sees(mask, g.sinks, keys.group(x) * 16 + 4 * kk + i % 4);
+            p[i] = seen ? exp2f(p[i] - m) : 0.f;
+            l += p[i];
+        }
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t x = 2 * tile + i / 16;
+            if (x >= keys.groups) break;
+            // the weight of key i for query c, from the lane that holds it
+            float w = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float v = __shfl(p[r], c + 16 * (i % 16 / 4));
+                w = r == i / 16 * 4 + i % 4 ? v : w;
+            }
+            if (!paged_sees(mask, g.sinks, keys.group(x) * 16 + i % 16)) continue;
+            const float* v = paged_group(g, b, keys.group(x), kvh) + paged_v_offset(g) + (i % 16) * row;
+#pragma unroll 1
+            for (uint32_t d = kk; d < g.head_dim; d += 4) o[d] = fmaf(w, v[d], o[d]);
+        }
     }
 }
 

@@ -51,6 +51,7 @@ bool check_paged_call(const BufferView& buffers, const PagedCall& given, Error* 
         return fail(err, Error::execution("heads must be a multiple of kv_heads"));
     if (D == 0 || D % 16 != 0 || D > 256)
         return fail(err, Error::unimplemented("paged operators need head_dim a multiple of 16 up to 256"));
+    if (H > 1024) return fail(err, Error::unimplemented("paged operators take at most 1024 heads"));
     if (kv.layers == 0 || c.op->layer >= kv.layers) return fail(err, Error::execution("layer is out of range"));
     if (c.kind != SL_PAGED_APPEND && !std::isfinite(c.op->scale))
         return fail(err, Error::execution("attention scale must be finite"));
@@ -110,7 +111,7 @@ bool check_paged_call(const BufferView& buffers, const PagedCall& given, Error* 
     return true;
 }
 
-bool check_paged_contents(const PagedCall& c, const PagedTables& t, PagedPlan* plan, Error* err) {
+bool check_paged_contents(const PagedCall& c, const PagedTables& t, uint32_t few, PagedPlan* plan, Error* err) {
     const sl_paged_kv& kv = *c.kv;
     const uint64_t B = c.tokens->batch, T = c.tokens->tokens, ps = kv.page_size, per = kv.pages_per_seq;
     const uint64_t capacity = per * ps;
@@ -133,13 +134,16 @@ bool check_paged_contents(const PagedCall& c, const PagedTables& t, PagedPlan* p
     };
     const auto pages = [&](uint64_t positions) { return (positions + ps - 1) / ps; };
     const char* const bad_id = "page id out of range";
-    uint64_t least = UINT64_MAX, most = 0, keys = 0;
+    uint64_t keys = 0;
+    const uint64_t group = c.op->heads / c.op->kv_heads;
     const uint32_t* shared = nullptr;  // the prefix's pages
     for (uint64_t b = 0; b < B; ++b) {
         const uint64_t L = t.seq_lens[b], n = starts[b + 1] - starts[b], end = L + n;
         if (n == 0) continue;
-        least = std::min(least, n);
-        most = std::max(most, n);
+        const uint64_t rows = n * group;
+        plan->rows_with_tokens += 1;
+        if (rows <= few) plan->few_rows += (rows + 15) / 16 * 16;  // (each row's blocks counted up)
+        else plan->many_rows += (rows + 15) / 16 * 16, plan->many_blocks += (rows + 255) / 256;
         if (c.kind == SL_PAGED_APPEND) {
             if (!in_range(b, L / ps, pages(end))) return fail(err, Error::execution(bad_id));
         } else if (c.kind == SL_PAGED_WINDOW) {
@@ -194,8 +198,6 @@ bool check_paged_contents(const PagedCall& c, const PagedTables& t, PagedPlan* p
         }
     }
     plan->most_keys = static_cast<uint32_t>(keys);
-    plan->most_rows = static_cast<uint32_t>(most);
-    plan->least_rows = least == UINT64_MAX ? 0 : static_cast<uint32_t>(least);
     return true;
 }
 
@@ -246,7 +248,7 @@ extern "C" sl_status sl_hip_validate_paged(const sl_buffer_desc* buffers, size_t
     } else {
         try {
             if (slhip::check_paged_call(view, c, &e))
-                (void)slhip::check_paged_contents(c, {row_starts, seq_lens, block_table}, &plan, &e);
+                (void)slhip::check_paged_contents(c, {row_starts, seq_lens, block_table}, 0, &plan, &e);
         } catch (...) {  // (no memory for the page marks)
             e = Error::out_of_memory(kv->num_pages);
         }

@@ -30,8 +30,9 @@ struct PagedCall {
 // What the launch is sized for.
 struct PagedPlan {
     uint32_t most_keys = 0;  // the most keys that one row's queries see
-    uint32_t most_rows = 0;  // the most new tokens of a row
-    uint32_t least_rows = 0; // the fewest of a row that has any
+    // query rows per KV head of the rows with up to `few` of them, of the others, and the others'
+    // blocks of 256 (each row's counted up); rows with tokens
+    uint64_t few_rows = 0, many_rows = 0, many_blocks = 0, rows_with_tokens = 0;
 };
 
 // A pointer that the operator cannot do without is null.
@@ -41,6 +42,6 @@ bool paged_argument_missing(const PagedCall& c);
 bool check_paged_call(const BufferView& buffers, const PagedCall& c, Error* err);
 // The contents of the row starts, lengths and block tables, after
 // check_paged_call.
-bool check_paged_contents(const PagedCall& c, const PagedTables& t, PagedPlan* plan, Error* err);
+bool check_paged_contents(const PagedCall& c, const PagedTables& t, uint32_t few, PagedPlan* plan, Error* err);
 
 }  // namespace slhip

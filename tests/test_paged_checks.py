@@ -73,6 +73,7 @@ def test_append_takes_queries_or_none_and_no_rotation():
     (dict(head_dim=0), DeviceError.unimplemented("paged operators need head_dim a multiple of 16 up to 256")),
     (dict(head_dim=72), DeviceError.unimplemented("paged operators need head_dim a multiple of 16 up to 256")),
     (dict(head_dim=272), DeviceError.unimplemented("paged operators need head_dim a multiple of 16 up to 256")),
+    (dict(heads=1026), DeviceError.unimplemented("paged operators take at most 1024 heads")),
     (dict(layer=2), execution("layer is out of range")),
     (dict(kv_heads=4), execution("page pool size does not match its layout")),
 ])
