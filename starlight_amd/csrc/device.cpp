@@ -1695,10 +1695,13 @@ PagedTokensArgs paged_tokens_args(Device* d, const PagedCall& c, const PagedPlan
     a.pages_per_seq = c.kv->pages_per_seq;
     a.window = c.window;
     a.sinks = c.sinks < 0x7fffffffu ? c.sinks : 0x7fffffffu;
-    a.most_keys = plan.most_keys;
+    a.few_keys = plan.few_keys;
+    a.many_keys = plan.many_keys;
     a.few_rows = static_cast<uint32_t>(plan.few_rows);
     a.many_rows = static_cast<uint32_t>(plan.many_rows);
     a.many_blocks = static_cast<uint32_t>(plan.many_blocks);
+    a.few_keys_in_all = plan.few_keys_in_all;
+    a.many_keys_in_all = plan.many_keys_in_all;
     a.rows_with_tokens = static_cast<uint32_t>(plan.rows_with_tokens);
     a.scale = c.op->scale;
     return a;

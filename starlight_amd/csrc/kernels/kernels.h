@@ -244,9 +244,10 @@ struct PagedTokensArgs {
     uint32_t num_pages, page_size, pages_per_seq;
     uint32_t window, sinks;  // window 0: none
     // what the launches are sized for (any other lengths and row starts stay right): the most
-    // keys that one row's queries see; the rows' query rows per KV head, of those with up to
-    // kPagedFewRows and of the others, and the others' blocks of 256
-    uint32_t most_keys, few_rows, many_rows, many_blocks, rows_with_tokens;
+    // keys that one row's queries see and the rows' query rows per KV head, of the rows with up to
+    // kPagedFewRows of them and of the others; the others' blocks of 256; both kinds' keys in all
+    uint32_t few_keys, many_keys, few_rows, many_rows, many_blocks, rows_with_tokens;
+    uint64_t few_keys_in_all, many_keys_in_all;
     float scale;
 };
 hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hipStream_t s);

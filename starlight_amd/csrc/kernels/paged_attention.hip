@@ -20,10 +20,11 @@
 //     same keys, its element e being column l % 16 of dim tile (J, e).
 // Every operand is two fp16 parts (paged_geo.h). Bound by HBM: splitting costs
 // about four vector instructions per K/V element, a fifth of the time the
-// element takes to arrive.
+// element takes to arrive. 16 rows of the 8B shape behind windows of 4,096 (493 MB): 89 us,
+// more than the rate of a large copy (4.9 TB/s).
 //
 // A tile whose values are not finite, or a result that is not a number, sends
-// the wave back over its tiles in plain f32 (slow_tile), where a key that a query
+// the wave back over its tiles in plain f32 (slow_tiles), where a key that a query
 // does not see contributes nothing whatever it holds.
 #include <algorithm>
 
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(64 * NW, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo 
     __shared__ __align__(16) float so[NW][M][OROW];
     __shared__ float sml[NW][M][2];
     PagedItem it;
-    if (!paged_item(g, g.item0 + blockIdx.x / g.kv_heads, blockIdx.y, M, &it)) return;  // block-uniform
+    if (!paged_item<false>(g, blockIdx.x / g.kv_heads, M, &it)) return;  // block-uniform
     const int tid = threadIdx.x, lane = tid % kWave, c = lane % 16, kk = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t kvh = blockIdx.x % g.kv_heads, D = g.head_dim, G = g.group;
@@ -144,13 +145,22 @@ __global__ __launch_bounds__(64 * NW, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo 
             if (kTogether) load_v(tile);
         }
         // scores
-        float most = 0.f;
+        float row[2] = {0.f, 0.f};  // the lane's two keys' largest values
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int j = 0; j < KS; ++j) most = max_abs(max_abs(most, kx[s][j][0]), kx[s][j][1]);
-        most = wave_max(most);
+            for (int j = 0; j < KS; ++j) row[s] = max_abs(max_abs(row[s], kx[s][j][0]), kx[s][j][1]);
+        float most = wave_max(fmaxf(row[0], row[1]));
         bad |= most == INFINITY;
+        const auto small = [&](float x) { return x < most * kApart && x != 0.f; };
+        if (__builtin_expect(__any(small(row[0]) || small(row[1])), 0)) {  // wave-uniform; seldom
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                row[s] = fmaxf(row[s], lane_xor16(row[s]));
+                row[s] = fmaxf(row[s], lane_xor32(row[s]));
+                bad |= small(row[s]);
+            }
+        }
         const int ke = part_exponent(most);
         const float kscale = power2(ke);
         v4f sc[2];
@@ -202,20 +212,53 @@ __global__ __launch_bounds__(64 * NW, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo 
         l = l * corr + sum;
         // values
         most = 0.f;
+        float least = INFINITY;
+        const auto largest = [&](int i) {  // of the lane's values of one key
+            float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+            for (int J = 0; J < DV; ++J) x = max_abs(x, vx[i][J]);
+            return x;
+        };
 #pragma unroll
-            for (int J = 0; J < DV; ++J) most = max_abs(most, vx[i][J]);
+        for (int i = 0; i < 8; ++i) {
+            const float x = largest(i);
+            most = fmaxf(most, x);
+            least = fminf(least, x == 0.f ? INFINITY : x);  // (zeros: past the last key)
+        }
         most = wave_max(most);
         bad |= most == INFINITY;
-        const int need = part_exponent(most);
-        const int ve = first ? need : min(need, oexp - kWeightTop);
-        // O's unit: the weights' 2^14 times the values' scale, lowered when larger values come
-        const float turn = first ? 0.f : power2(ve + kWeightTop - oexp);
+        if (__builtin_expect(__any(least < most * kApart), 0)) {  // wave-uniform; seldom
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bad |= row_apart<16>(largest(i), most);
+#pragma unroll
+            for (int J = 0; J < DV; ++J) {
+                const auto joined = [&](auto at) {  // of a column
+                    float x = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x = fmaxf(x, fabsf(at(vx[i][J])));
+                    x = fmaxf(x, lane_xor16(x));
+                    return fmaxf(x, lane_xor32(x));
+                };
+                const float x = joined([](float4 v) { return v.x; }), y = joined([](float4 v) { return v.y; }),
+                            z = joined([](float4 v) { return v.z; }), w = joined([](float4 v) { return v.w; });
+                const float limit = most * kApart;
+                bad |= (x < limit && x != 0.f) || (y < limit && y != 0.f) || (z < limit && z != 0.f) ||
+                       (w < limit && w != 0.f);
+            }
+        }
+        // O's unit: the weights' 2^14 times the values' scale
+        const int need = part_exponent(most), held = first ? need : oexp - kWeightTop;
+        const int ve = most != 0.f && (need < held || need > held + kUnitSlack) ? need : held;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= corr;
+        if (__builtin_expect(ve != held, 0)) {  // wave-uniform
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] = __builtin_ldexpf(o[d][i], ve - held);
+        }
         first = false;
         oexp = ve + kWeightTop;
-        #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= corr * turn;
         const Parts w = to_parts(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], power2(kWeightTop));
         const float vscale = power2(ve);
 #pragma unroll
@@ -276,13 +319,9 @@ __global__ __launch_bounds__(64 * NW, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo 
             if (f != 0.f) fma4(acc, f, *reinterpret_cast<const float4*>(&so[w][x][d]));
         }
         const uint64_t at = row_of(it.r0 + x);
-        if (g.slots == 1) {
-            store4(g.out + at * D + d, scaled4(acc, 1.0f / sum), aligned);
-        } else {
-            const uint64_t slot = at * g.slots + it.slot;
-            *reinterpret_cast<float4*>(g.part + slot * D + d) = acc;
-            if (d == 0) g.ml[slot] = make_float2(mm, sum);
-        }
+        if (paged_direct(g)) store4(g.out + at * D + d, scaled4(acc, 1.0f / sum), aligned);
+        else *reinterpret_cast<float4*>(g.part + (at * g.slots + it.slot) * D + d) = acc;
+        if (d == 0) paged_state(g, it, at, mm, sum);
     }
 }
 
@@ -304,20 +343,27 @@ __global__ __launch_bounds__(256) void paged_merge(PagedGeo g) {
     const uint64_t at = row0 + x;
     const float* const part = g.part + at * S * g.head_dim + 4 * c;
     float4 v[U];
+    uint32_t last = S - 1;
     const auto load = [&](uint32_t s0) {  // (past the last they re-read it, with weight 0)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            v[u] = *reinterpret_cast<const float4*>(part + static_cast<uint64_t>(min(s0 + u, S - 1)) * g.head_dim);
+            v[u] = *reinterpret_cast<const float4*>(part + static_cast<uint64_t>(min(s0 + u, last)) * g.head_dim);
     };
     for (uint32_t i = tid; i < here * S; i += 256) ml[i / S][i % S] = g.ml[row0 * S + i];
-    load(0);
+    if (g.uneven == 0) load(0);
     __syncthreads();
     float mm = -INFINITY;
-    for (uint32_t s = 0; s < S; ++s) mm = fmaxf(mm, ml[x][s].x);
+    uint32_t count = S;  // the row's partials
+    if (g.uneven != 0) {
+        for (count = 0; count < S && !(ml[x][count].y < 0.f);) ++count;
+        last = max(count, 1u) - 1;
+        load(0);
+    }
+    for (uint32_t s = 0; s < count; ++s) mm = fmaxf(mm, ml[x][s].x);
     __syncthreads();
     // each of a row's threads its share of the weights (a NaN maximum keeps its sum's NaN)
     if (tid / d4 < here)
-        for (uint32_t s = c; s < S; s += d4) {
+        for (uint32_t s = c; s < count; s += d4) {
             const float2 p = ml[x][s];
             const float f = p.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p.x - mm);
             ml[x][s] = make_float2(f, p.y * f);
@@ -325,18 +371,18 @@ __global__ __launch_bounds__(256) void paged_merge(PagedGeo g) {
     __syncthreads();
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s0 = 0; s0 < S; s0 += U) {
+    for (uint32_t s0 = 0; s0 < count; s0 += U) {
         if (s0 != 0) load(s0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (s0 + u >= S) continue;
+            if (s0 + u >= count) continue;
             const float2 p = ml[x][s0 + u];
             l += p.y;
             // (an empty partial's values are zeros)
             fma4(o, p.x, v[u]);
         }
     }
-    if (tid / d4 < here)
+    if (tid / d4 < here && count != 0)
         store4(g.out + at * g.head_dim + 4 * c, scaled4(o, 1.0f / l), g.aligned != 0);
 }
 
@@ -374,17 +420,16 @@ PagedGeo paged_geometry(const PagedTokensArgs& a) {
 
 constexpr uint32_t kBlockRows = 16;  // query rows of a paged_rows block
 
-// Items of a launch with `per` query rows each: the shared ones, and the rows' own.
-uint64_t shared_items(const PagedGeo& g, uint64_t per) {
-    return (static_cast<uint64_t>(g.tokens) * g.group + per - 1) / per;
+// Items with `per` query rows each: of all tokens together, and row by row.
+uint32_t items_together(const PagedGeo& g, uint64_t per) {
+    return static_cast<uint32_t>((static_cast<uint64_t>(g.tokens) * g.group + per - 1) / per);
 }
-uint64_t own_items(const PagedGeo& g, uint64_t per) {
-    return static_cast<uint64_t>(g.tokens) * g.group / per + g.batch;
+uint32_t items_by_row(const PagedGeo& g, uint64_t per) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(g.tokens) * g.group / per + g.batch);
 }
 
-hipError_t launch_rows(const PagedGeo& g, uint64_t items, hipStream_t s) {
-    const uint32_t splits = std::max(g.item0 < g.shared_items ? g.shared_splits : 0, g.splits);
-    const dim3 grid(static_cast<unsigned>(items * g.kv_heads), splits);
+hipError_t launch_rows(const PagedGeo& g, hipStream_t s) {
+    const unsigned grid = paged_blocks(g);
     const bool exact = g.head_dim % 64 == 0;
 #define SL_ROWS(DV, NW)                                               \
     do {                                                              \
@@ -420,61 +465,114 @@ bool place_partials(PagedGeo* g, uint32_t slots, const Workspace& ws) {
 }
 
 // Key splits for `blocks` blocks of equal work, one per CU at a time, whose keys take `steps`
-// steps (256 keys of paged_rows, 64 of paged_tiles): a round of blocks costs its steps and
-// `fixed` more, partials a step or two. (1 for a batch that fills the chip by itself; 2 for
-// blocks that would leave a second round half empty.)
-uint32_t splits_for(uint64_t blocks, uint64_t steps, double fixed) {
+// steps (256 keys of paged_rows, 64 of paged_tiles), and the time they take: a round of blocks
+// costs its steps and `fixed` more, partials a step, and `partial` for each block's. (1 for a
+// batch that fills the chip by itself; 2 for blocks that would leave a second round half empty.)
+// Of the launch's blocks, `launched` per split with those that find nothing to do, there may be
+// 2^23.
+struct SplitCosts {
+    double step_us, fixed, partial;
+};
+struct Splits {
+    uint32_t n;
+    double us;
+};
+Splits splits_for(uint64_t blocks, uint64_t launched, uint64_t steps, const SplitCosts& cost) {
     const uint64_t cus = compute_units();
-    if (blocks == 0) return 1;
-    uint32_t best = 1;
-    double least = 0.0;
-    for (uint32_t n = 1; n <= kMergeSlots / 2 && n <= steps; ++n) {
+    Splits best{1, 0.0};
+    for (uint32_t n = 1; n <= kMergeSlots / 2 && n <= std::max<uint64_t>(steps, 1) && n * launched < 1u << 23; ++n) {
         const double rounds = static_cast<double>((blocks * n + cus - 1) / cus);
-        const double cost = rounds * (static_cast<double>(steps) / n + fixed) + (n > 1 ? 1.5 : 0.0);
-        if (n == 1 || cost < least) {
-            least = cost;
-            best = n;
-        }
+        const double us = cost.step_us * (rounds * (static_cast<double>(steps) / n + cost.fixed) +
+                                          (n > 1 ? 1.0 + static_cast<double>(blocks * n) * cost.partial : 0.0));
+        if (n == 1 || us < best.us) best = {n, us};
     }
     return best;
 }
-constexpr double kRowsFixed = 0.5, kTilesFixed = 4.0;  // measured: about 4 us and 20 us
 
-// Bytes of K and V that sharing has to save, and query rows up to which the shared part is
-// paged_rows' (8B shapes, 16 rows over a prefix of 2,000: 27.9 us, with paged_tiles 42.0; 34 tokens
-// of 8 rows over 4,096: 54.1, with paged_tiles 52.4; 64 over 16,384: 262, with paged_tiles 143).
-constexpr uint64_t kSharingPays = 24ull << 20;
-constexpr uint64_t kSharedFewRows = 64;
+// Measured at head_dim 128 (at 64 both steps take two thirds; what counts is their relation). Rows
+// that read much from HBM take at least that long. What the choice between the two goes by, all
+// rows to paged_rows (all to paged_tiles), 8B shape:
+//   1 row of 32, 128, 256, 360 new tokens at 0: 7.8, 9.8, 21.0, 33.0 us (15.5, 26.8, 34.7, 37.9),
+//   of 32, 64 at 2,000: 21.8, 32.2 (31.5, 38.0), of 8, 32 at 16,000: 40.5, 101 (52.4, 60.6);
+//   8 rows of 4, 8, 16 at 2,000: 31.9, 39.6, 55.5 (48.7, 50.5, 53.0); 4 rows of 8 at 16,000: 120
+//   (146), of 180 at 0: 51.0 (31.8); 16 rows of 40 at 0: 35.9 (20.8).
+// (It takes the other one for 360 at 0, 64 at 2,000 and 16 rows of 20 at 100, 26.2 us and not 20.2.)
+constexpr SplitCosts kRowsCosts{6.0, 0.5, 0.002}, kTilesCosts{4.5, 4.0, 0.006};
+double read_us(const PagedGeo& g, uint64_t keys) {
+    return static_cast<double>(keys) * g.kv_heads * g.head_dim * 8 / 4.9e6 * (g.head_dim > 64 ? 1.0 : 1.5);
+}
+
+// Splits of paged_rows for `query_rows` in blocks that see up to `keys` keys.
+Splits rows_splits(const PagedGeo& g, uint64_t query_rows, uint64_t launched, uint64_t keys) {
+    return splits_for((query_rows + kBlockRows - 1) / kBlockRows * g.kv_heads, launched * g.kv_heads, (keys + 255) / 256,
+                      kRowsCosts);
+}
+Splits tiles_splits(const PagedGeo& g, uint64_t blocks, uint64_t launched, uint64_t keys) {
+    return splits_for(blocks * g.kv_heads, launched * g.kv_heads, (keys + 63) / 64, kTilesCosts);
+}
 
 }  // namespace
 
 hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hipStream_t s) {
     if (a.tokens == 0) return hipSuccess;
     PagedGeo g = paged_geometry(a);
-    // rows of a sequence's tokens go to paged_rows up to kPagedFewRows query rows, above to
-    // paged_tiles: which launches there are, and their splits, follow the row starts of this call;
-    // each launch takes the rows that are its own when it runs
-    const bool tiles = a.many_rows != 0 && g.head_dim <= 128, some = !tiles || a.few_rows != 0;
-    const uint64_t few = a.few_rows + (tiles ? 0 : a.many_rows);
-    uint32_t splits = 1;
-    if (some) splits = splits_for((few + kBlockRows - 1) / kBlockRows * g.kv_heads, (a.most_keys + 255) / 256, kRowsFixed);
-    if (tiles)
-        splits = splits_for(static_cast<uint64_t>(a.many_blocks) * g.kv_heads, (a.most_keys + 63) / 64, kTilesFixed);
-    if (splits > 1 && place_partials(&g, splits, ws)) g.splits = splits;
+    // All of the call's rows to paged_rows, or those with up to kPagedFewRows query rows, the
+    // others to paged_tiles: which launches there are, and their splits, follow the row starts of
+    // this call; each launch takes the rows that are its own when it runs.
+    PagedGeo r = g, t = g;
+    // (a block's queries see their windows and the positions between them)
+    const auto seen = [&](uint64_t keys, uint32_t rows) {
+        return std::min<uint64_t>(keys, uint64_t{g.window} + rows / g.group + g.sinks);
+    };
+    r.own_items = items_by_row(g, kBlockRows);
+    t.own_items = items_by_row(g, kTileRows);
+    const uint32_t most_few = std::min(g.batch * (kPagedFewRows / kBlockRows), r.own_items);
+    bool some = true, tiles = false;
+    Splits rs = rows_splits(g, static_cast<uint64_t>(a.few_rows) + a.many_rows, r.own_items,
+                            std::max<uint64_t>(a.few_keys, seen(a.many_keys, kBlockRows)));
+    Splits ts{1, 0.0};
+    if (a.many_rows != 0 && g.head_dim <= 128) {
+        Splits few{1, 0.0};
+        if (a.few_rows != 0) {
+            few = rows_splits(g, a.few_rows, most_few, a.few_keys);
+            few.us = std::max(few.us, read_us(g, a.few_keys_in_all));
+        }
+        ts = tiles_splits(g, a.many_blocks, t.own_items, seen(a.many_keys, kTileRows));
+        if (few.us + ts.us < std::max(rs.us, read_us(g, a.few_keys_in_all + a.many_keys_in_all))) {
+            rs = few;
+            tiles = true;
+            some = a.few_rows != 0;
+        } else {
+            ts.n = 1;
+        }
+        if (tiles && some) {
+            r.rows_upto = t.rows_over = kPagedFewRows;
+            r.own_items = most_few;
+        }
+    }
+    // (as many splits as the workspace has room for)
+    const uint64_t room = ws.floats / (static_cast<uint64_t>(g.tokens) * g.heads * (g.head_dim + 2) + 64);
+    const auto fit = [&](uint32_t n) { return static_cast<uint32_t>(std::min<uint64_t>(n, std::max<uint64_t>(room, 1))); };
+    const uint32_t slots = fit(std::max(rs.n, ts.n));
+    if (slots > 1 && place_partials(&g, slots, ws)) {
+        r.splits = fit(rs.n);
+        t.splits = fit(ts.n);
+        g.uneven = some && tiles && r.splits != t.splits;
+        r.slots = t.slots = slots;
+        r.ml = t.ml = g.ml;
+        r.part = t.part = g.part;
+    }
     hipError_t e = hipSuccess;
-    if (some) {
-        PagedGeo x = g;
-        if (tiles) x.rows_upto = kPagedFewRows;
-        e = launch_rows(x, own_items(g, kBlockRows), s);
-    }
-    if (e == hipSuccess && tiles) {
-        PagedGeo x = g;
-        if (some) x.rows_over = kPagedFewRows;
-        e = launch_paged_tiles(x, own_items(g, kTileRows), s);
-    }
+    if (some) e = launch_rows(r, s);
+    if (e == hipSuccess && tiles) e = launch_paged_tiles(t, s);
     if (e == hipSuccess && g.slots > 1) e = launch_merge(g, s);
     return e;
 }
+
+// Bytes of K and V that sharing has to save: 4 rows of the 8B shape over 500, 1,000, 2,000
+// positions (12, 24, 48 MiB) take 14.2, 15.0, 16.4 us by themselves, 19.8, 15.3, 16.0 shared;
+// 16 over 208 (25 MiB) 12.0 and 14.5; 16 over 2,000 33.0 and 23.0.
+constexpr uint64_t kSharingPays = 32ull << 20;
 
 hipError_t launch_paged_prefix(const PagedTokensArgs& a, uint32_t prefix, const Workspace& ws, hipStream_t s) {
     if (a.tokens == 0) return hipSuccess;
@@ -484,24 +582,25 @@ hipError_t launch_paged_prefix(const PagedTokensArgs& a, uint32_t prefix, const 
     // on their own (what they share then comes from the caches).
     const uint64_t saved = static_cast<uint64_t>(prefix) * (a.rows_with_tokens - 1) * g.kv_heads * g.head_dim * 8;
     if (saved < kSharingPays) return launch_paged_window(a, ws, s);
-    const bool tiles = g.head_dim <= 128 && rows > kSharedFewRows;
-    const uint64_t shared = shared_items(g, tiles ? kTileRows : kBlockRows);
-    const uint64_t few = a.few_rows + a.many_rows;
-    g.shared_splits = tiles ? splits_for(shared * g.kv_heads, (prefix + 63) / 64, kTilesFixed)
-                            : splits_for(shared * g.kv_heads, (prefix + 255) / 256, kRowsFixed);
-    g.splits = splits_for((few + kBlockRows - 1) / kBlockRows * g.kv_heads, (a.most_keys - prefix + 255) / 256, kRowsFixed);
+    const uint32_t by_rows = items_together(g, kBlockRows), by_tiles = items_together(g, kTileRows);
+    const Splits rs = rows_splits(g, rows, 2ull * by_rows, prefix), ts = tiles_splits(g, by_tiles, 2ull * by_tiles, prefix);
+    const bool tiles = g.head_dim <= 128 && ts.us < rs.us;
+    g.shared_splits = tiles ? ts.n : rs.n;
+    g.own_items = items_by_row(g, kBlockRows);
+    g.splits = rows_splits(g, static_cast<uint64_t>(a.few_rows) + a.many_rows, 2ull * g.own_items,
+                           std::max(a.few_keys, a.many_keys) - prefix).n;
     if (!place_partials(&g, g.shared_splits + g.splits, ws)) return launch_paged_window(a, ws, s);
     g.prefix = prefix;
-    g.shared_items = static_cast<uint32_t>(shared);
     hipError_t e = hipSuccess;
     if (tiles) {
-        e = launch_paged_tiles(g, shared, s);
-        // (the rows' own items are counted in paged_rows' measure)
-        g.item0 = g.shared_items;
-        if (e == hipSuccess) e = launch_rows(g, own_items(g, kBlockRows), s);
+        PagedGeo x = g;
+        x.shared_items = by_tiles;
+        x.own_items = 0;
+        e = launch_paged_tiles(x, s);
     } else {
-        e = launch_rows(g, shared + own_items(g, kBlockRows), s);  // both kinds beside one another
+        g.shared_items = by_rows;  // both kinds beside one another
     }
+    if (e == hipSuccess) e = launch_rows(g, s);
     if (e == hipSuccess) e = launch_merge(g, s);
     return e;
 }

@@ -26,20 +26,29 @@ struct PagedGeo {
     uint32_t page16, pages_per_seq, num_pages;  // page16: 16-position groups per page,
     uint32_t page_shift;                        // its logarithm, or 32 where it is no power of two
     uint32_t window, sinks;                     // window 0xffffffff: none
-    // Items of a launch: first shared_items of them (from item0 on) are all tokens' queries over
-    // the positions below `prefix`, which lie in the same pages for every row; the others are each
-    // row's queries over its positions from `prefix` on.
-    uint32_t prefix, shared_items, item0;
-    uint32_t shared_splits, splits, slots;  // key splits of the two kinds; partials per query row, the shared first
+    // A launch's units of work, kv_heads blocks each: own_items x splits (own_items at least as
+    // many as there are), each row's queries over its positions from `prefix` on (first: their
+    // lengths differ); then shared_items x
+    // shared_splits, all tokens' queries over the positions below `prefix`, which lie in the same
+    // pages for every row.
+    uint32_t prefix, shared_items, shared_splits, own_items, splits;
+    // Partials a query row has room for, the shared first. A row that leaves the later of
+    // them ends its list with a sum of -1 (splits 1 and no prefix: at once, its result is written).
+    uint32_t slots;
+    uint32_t uneven;                            // rows have fewer partials than slots
     uint32_t aligned;                           // q and out are 16-byte aligned
     uint32_t rows_over, rows_upto;              // rows with rows_over < query rows <= rows_upto, the others exit
     float scale;
 };
 
 // paged_tiles.hip: the form for many query rows per KV head, kTileRows per block, head_dim up to
-// 128. One launch over `items` items.
+// 128.
 constexpr uint32_t kTileRows = 256;
-hipError_t launch_paged_tiles(const PagedGeo& g, uint64_t items, hipStream_t s);
+hipError_t launch_paged_tiles(const PagedGeo& g, hipStream_t s);
+
+inline unsigned paged_blocks(const PagedGeo& g) {
+    return (g.shared_items * g.shared_splits + g.own_items * g.splits) * g.kv_heads;
+}
 
 namespace {
 
@@ -50,23 +59,62 @@ struct PagedItem {
     uint32_t begin, end, splits, split, slot;
 };
 
-// Item x of a grid with M query rows per item. Row b has the items from
-// starts[b] * group / M + b on (after the shared ones): at least as many as its query rows
-// need, and found from starts alone. Every wave of a block comes to the same answer. False:
-// nothing to do.
-__device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t item, uint32_t split, uint32_t M, PagedItem* it) {
-    const uint32_t lane = threadIdx.x % kWave;
-    it->split = split;
-    if (item < g.shared_items) {
-        if (split >= g.shared_splits) return false;
+// The rows b0 .. b0 + 63, one per lane: a row's tokens and length, how many items of M query
+// rows it makes here (none where its kind is another launch's), and how many the rows before it
+// in the 64 make.
+struct PagedRow {
+    uint32_t start, n, len, items, before;
+};
+__device__ __forceinline__ PagedRow paged_row(const PagedGeo& g, uint32_t b0, uint32_t M) {
+    const uint32_t lane = threadIdx.x % kWave, b = min(b0 + lane, g.batch - 1);
+    // (bounds that hold for checked buffers, and keep a replayed launch in range whatever
+    // they hold then)
+    const uint32_t capacity = g.pages_per_seq * g.page16 * 16, next = min(g.starts[b + 1], g.tokens);
+    PagedRow r;
+    r.start = min(g.starts[b], next);
+    r.len = min(g.lens[b], capacity);
+    r.n = min(next - r.start, capacity - r.len);
+    const uint32_t rows = r.n * g.group;
+    const bool mine = b0 + lane < g.batch && rows > g.rows_over && rows <= g.rows_upto;
+    r.items = mine ? (rows + M - 1) / M : 0;
+    const uint64_t one = __ballot(r.items != 0);
+    if (__ballot(r.items > 1) == 0) {  // wave-uniform
+        r.before = __popcll(one & ((1ull << lane) - 1));
+    } else {
+        uint32_t sum = r.items;
+#pragma unroll
+        for (uint32_t d = 1; d < kWave; d *= 2) {
+            const uint32_t below = __shfl_up(sum, d);
+            sum += lane >= d ? below : 0;
+        }
+        r.before = sum - r.items;
+    }
+    return r;
+}
+__device__ __forceinline__ uint32_t paged_row_items(const PagedRow& r) {  // of the 64 rows
+    return __builtin_amdgcn_readlane(r.before + r.items, kWave - 1);
+}
+
+// Unit `unit` of a launch with M query rows per item (LAST_FIRST: the own items from the last to
+// the first). The items are counted from the row starts, so those that there are lie side by side
+// whatever the rows: blocks without work between the others would leave some of the chip's
+// shader engines, which are given blocks in turn, with one block more than they have CUs
+// (256 blocks of paged_tiles 98 us, not 70). Every wave of a block comes to the same answer.
+// False: nothing to do.
+template <bool LAST_FIRST>
+__device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t unit, uint32_t M, PagedItem* it) {
+    const uint32_t own_units = g.own_items * g.splits;
+    if (unit >= own_units) {
+        unit -= own_units;
+        it->split = unit / g.shared_items;
         it->begin = 0;
         it->end = g.prefix;
         it->splits = g.shared_splits;
-        it->slot = split;
+        it->slot = it->split;
         // (the first row that has a token: its table names the shared pages)
         uint32_t row = 0;
         for (uint32_t b0 = 0; b0 < g.batch; b0 += kWave) {
-            const uint32_t b = b0 + lane;
+            const uint32_t b = b0 + threadIdx.x % kWave;
             const uint64_t some = __ballot(b < g.batch && g.starts[min(b, g.batch - 1) + 1] != 0);
             if (some != 0) {
                 row = b0 + static_cast<uint32_t>(__builtin_ctzll(some));
@@ -77,43 +125,40 @@ __device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t item, uin
         it->len = g.prefix;
         it->n = g.tokens;
         it->t0 = 0;
-        it->r0 = item * M;
+        it->r0 = (unit - it->split * g.shared_items) * M;
         return it->r0 < it->n * g.group;
     }
-    if (split >= g.splits) return false;
-    const uint32_t x = item - g.shared_items;
+    PagedRow r = paged_row(g, 0, M);
+    uint32_t x = unit, first = 0;
+    it->split = 0;
+    if (LAST_FIRST || g.splits != 1) {
+        uint32_t total = paged_row_items(r);
+        for (uint32_t b0 = kWave; b0 < g.batch; b0 += kWave) total += paged_row_items(paged_row(g, b0, M));
+        if (unit >= total * g.splits) return false;
+        if (g.splits != 1) {
+            it->split = unit / total;
+            x -= it->split * total;
+        }
+        if (LAST_FIRST) x = total - 1 - x;
+    }
+    for (uint32_t here = paged_row_items(r); x >= here && first + kWave < g.batch; here = paged_row_items(r)) {
+        x -= here;
+        first += kWave;
+        r = paged_row(g, first, M);
+    }
+    const uint64_t found = __ballot(x >= r.before && x < r.before + r.items);
+    if (found == 0) return false;
+    const int at = __builtin_ctzll(found);
     it->begin = g.prefix;
     it->end = 0xffffffffu;
     it->splits = g.splits;
-    it->slot = (g.prefix != 0 ? g.shared_splits : 0) + split;
-    uint32_t row = 0, start = 0, next = 0, len = 0, base = 0;
-    for (uint32_t b0 = 0; b0 < g.batch; b0 += kWave) {
-        const uint32_t b = min(b0 + lane, g.batch - 1);
-        const uint32_t s = g.starts[b], e = g.starts[b + 1], l = g.lens[b];
-        const uint32_t at = s * g.group / M + b;
-        const uint64_t below = __ballot(b0 + lane < g.batch && at <= x);
-        if (below == 0) break;
-        const int last = 63 - __builtin_clzll(below);
-        row = b0 + last;
-        start = __builtin_amdgcn_readlane(s, last);
-        next = __builtin_amdgcn_readlane(e, last);
-        len = __builtin_amdgcn_readlane(l, last);
-        base = __builtin_amdgcn_readlane(at, last);
-        if (below != ~0ull) break;
-    }
-    // (bounds that hold for checked buffers, and keep a replayed launch in
-    // range whatever they hold then)
-    next = min(next, g.tokens);
-    start = min(start, next);
-    const uint32_t capacity = g.pages_per_seq * g.page16 * 16;
-    len = min(len, capacity);
-    it->b = __builtin_amdgcn_readfirstlane(row);
-    it->t0 = start;
-    it->n = min(next - start, capacity - len);
-    it->len = len;
-    it->r0 = (x - base) * M;
-    const uint32_t rows = it->n * g.group;
-    return it->r0 < rows && rows > g.rows_over && rows <= g.rows_upto;
+    it->slot = (g.prefix != 0 ? g.shared_splits : 0) + it->split;
+    it->b = first + at;
+    it->t0 = __builtin_amdgcn_readlane(r.start, at);
+    it->n = __builtin_amdgcn_readlane(r.n, at);
+    it->len = __builtin_amdgcn_readlane(r.len, at);
+    it->r0 = (x - __builtin_amdgcn_readlane(r.before, at)) * M;
+    return true;
 }
 
 // The keys that the query rows r0 .. r0 + count - 1 of an item see, as a list of
@@ -136,6 +181,20 @@ __device__ __forceinline__ PagedKeys paged_keys(const PagedGeo& g, const PagedIt
     const uint32_t last = (k.end + 15) / 16;
     k.groups = k.sink_groups + (last > k.first_group ? last - k.first_group : 0);
     return k;
+}
+
+// Whether the launch writes results, not partials.
+__device__ __forceinline__ bool paged_direct(const PagedGeo& g) { return g.splits == 1 && g.prefix == 0; }
+// The partial `slot` of a query row (token and head), its values written by the caller; `m` and
+// `l` are not looked at for a result.
+__device__ __forceinline__ void paged_state(const PagedGeo& g, const PagedItem& it, uint64_t row, float m, float l) {
+    float2* const ml = g.ml + row * g.slots;
+    if (paged_direct(g)) {
+        if (g.slots > 1) ml[0] = make_float2(0.f, -1.f);
+        return;
+    }
+    ml[it.slot] = make_float2(m, l);
+    if (g.prefix == 0 && it.split == 0 && g.splits < g.slots) ml[g.splits] = make_float2(0.f, -1.f);
 }
 
 // Which keys a query at `position` sees: j < end and (j >= low or j < sinks).
@@ -205,7 +264,26 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
+// So rows (one position's keys or values) that share a scale have to be of like magnitude, for a
+// query may see the small ones and not the large, and so have the values' columns, each a result
+// of its own: where one of them, not all zero, is kApart below the largest value beside it,
+// the plain form takes over.
 constexpr int kPartTop = 14;  // the largest value's exponent after scaling
+constexpr float kApart = 0x1p-16f;
+// O's unit is lowered as larger values come, and raised again by more than this.
+constexpr int kUnitSlack = 8;
+// Whether one of the rows that N lanes hold together is such a one; m: the largest of the lane's values.
+template <int N>
+__device__ __forceinline__ bool row_apart(float m, float most) {
+    const uint64_t small = __ballot(m < most * kApart), zero = __ballot(m == 0.f);
+    bool apart = false;
+#pragma unroll
+    for (int at = 0; at < 64; at += N) {
+        const uint64_t lanes = ((1ull << N) - 1) << at;
+        apart |= (small & lanes) == lanes && (zero & lanes) != lanes;
+    }
+    return apart;
+}
 
 // The scale's exponent for a block whose largest magnitude is `most` (finite):
 // between -113 and 60, so that the scales of two operands can be multiplied.

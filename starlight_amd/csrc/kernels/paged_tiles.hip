@@ -17,12 +17,18 @@
 //     4 (l % 32) of the keys 8 (i / 4) + 4 (l / 32) + i % 4, i < 8, of a group holds, for
 //     each e, row l % 32 of the dim tile e whose row r is dim 4 r + e.
 // The softmax state is per lane, the sum of a query's weights added up over its two
-// lanes at the end. O^T is kept in units of 2^-oexp, which all waves of a block
-// lower together when a stage brings larger values.
+// lanes at the end. O^T is kept in units of 2^-oexp, which follows the groups' values,
+// so that the weights' fp16 parts keep their bits whatever a query's other keys hold.
 //
-// Bound by the matrix cores: three fp16 products per product, so 2.5 / 3 PFLOP/s at
-// best; splitting costs 130 vector instructions per wave and stage, the softmax
-// about 12 per weight.
+// Bound by the matrix cores and by the vector work between their products (splitting,
+// and about 12 instructions per weight), which overlap only in part: a stage takes about
+// 11,000 cycles where its products take 6,100. 2,048 tokens at 6,000 of the 8B shape behind
+// a window of 4,096: 410 us, 1.0 PFLOP/s of fp16 products, three of them per product
+// (hipBLASLt's 8192^3 reaches 1.08). The scores of a whole stage before its softmax, not of
+// 32 keys at a time: 128 us, not 132, for a prompt of 3,001 of the 1B shape, and 134 with the
+// looks at how far the rows and groups lie apart.
+// No better: two tiles of 32 queries per wave, blocks of 4 waves, stages of 32 keys, raised wave
+// priorities; four waves per SIMD at head_dim 64 spill and take 160 us for that prompt.
 #include "paged_geo.h"
 
 namespace slhip {
@@ -35,6 +41,7 @@ constexpr int NW = 8;  // waves per block
 // Weights are up to 2^kSlack, 2^(kSlack + kTileTop) as fp16 parts.
 constexpr float kSlack = 8.f;
 constexpr int kTileTop = 7;
+constexpr int kNoUnit = 1000;  // of a group whose values are all zero
 
 template <int DV>
 struct TileShape {
@@ -56,8 +63,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
     __shared__ int flags;
     PagedItem it;
     // (the last query rows, which see the most keys, first)
-    const uint32_t items = gridDim.x / g.kv_heads;
-    if (!paged_item(g, g.item0 + items - 1 - blockIdx.x / g.kv_heads, blockIdx.y, kTileRows, &it)) return;  // block-uniform
+    if (!paged_item<true>(g, blockIdx.x / g.kv_heads, kTileRows, &it)) return;  // block-uniform
     const int tid = threadIdx.x, lane = tid % kWave, c = lane % 32, hh = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t kvh = blockIdx.x % g.kv_heads, D = g.head_dim, G = g.group;
@@ -124,10 +130,42 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
         }
     };
     const auto stage_out = [&](int half) {
-        float most = 0.f;
+        const auto value = [&](int i, int d) -> float {  // key i's dim d, of the lane's V
+            const float4 q = x[VW * i / 4];
+            const int e4 = DV == 2 ? d : 2 * (i % 2) + d;
+            return e4 == 0 ? q.x : e4 == 1 ? q.y : e4 == 2 ? q.z : q.w;
+        };
+        float most = 0.f, least = INFINITY;
+        // (two keys' values in one float4)
+        const auto pair = [&](int u) { return make_float2(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w))); };
 #pragma unroll
-        for (int u = 0; u < KV4; ++u) most = max_abs(most, x[u]);
+        for (int u = 0; u < KV4; ++u) {
+            const float2 p = pair(u);
+            const float both = fmaxf(p.x, p.y);
+            most = fmaxf(most, both);
+            least = fminf(least, DV == 1 && !loads_k ? fminf(p.x, p.y) : both);
+        }
         most = wave_max(most);
+        uint32_t apart = 0;
+        if (__builtin_expect(__any(least < most * kApart), 0)) {  // wave-uniform; seldom, but for rows of zeros
+#pragma unroll
+            for (int u = 0; u < KV4; ++u) {
+                const float2 p = pair(u);
+                if (loads_k) apart |= row_apart<F>(fmaxf(p.x, p.y), most);
+                else if constexpr (DV == 2) apart |= row_apart<32>(fmaxf(p.x, p.y), most);
+                else apart |= row_apart<32>(p.x, most) || row_apart<32>(p.y, most);
+            }
+            if (!loads_k) {
+#pragma unroll
+                for (int d = 0; d < VW; ++d) {
+                    float column = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) column = fmaxf(column, fabsf(value(i, d)));
+                    column = fmaxf(column, lane_xor32(column));
+                    apart |= __any(column < most * kApart && column != 0.f);
+                }
+            }
+        }
         const int e = part_exponent(most);
         const float scale = power2(e);
         uint8_t* const base = lds + half * Shape::STAGE;
@@ -144,11 +182,6 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
             }
         } else {
             uint8_t* const to = base + 2 * Shape::KPART + mine * Shape::VGROUP + 16 * lane;
-            const auto value = [&](int i, int d) -> float {
-                const float4 q = x[VW * i / 4];
-                const int e4 = DV == 2 ? d : 2 * (i % 2) + d;
-                return e4 == 0 ? q.x : e4 == 1 ? q.y : e4 == 2 ? q.z : q.w;
-            };
 #pragma unroll
             for (int d = 0; d < VW; ++d) {
                 const Parts p = to_parts(value(0, d), value(1, d), value(2, d), value(3, d), value(4, d), value(5, d),
@@ -158,8 +191,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
             }
         }
         if (lane == 0) {
-            exps[half][loads_k ? 0 : 1][mine] = e;
-            if (most == INFINITY) flags = 1;
+            exps[half][loads_k ? 0 : 1][mine] = loads_k || most != 0.f ? e : kNoUnit;
+            if (apart || most == INFINITY) flags = 1;
         }
     };
 
@@ -208,7 +241,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
-    int oexp = 1000;  // (above any stage's: set by the first)
+    int oexp = kNoUnit;  // (none yet)
     if (stage0 < stages) {
         stage_out(0);
         if (!loads_k && stage0 + 1 < stages) load_next(stage0 + 1);
@@ -218,87 +251,98 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
     for (uint32_t stage = stage0; stage < stages; ++stage) {
         const int half = (stage - stage0) & 1;
         const bool more = stage + 1 < stages;
-        // The waves w and w + 4 split at the two ends of a stage. They share a SIMD, which prefers the older one: its products run while the other splits, and the
-        // other's while it is at its softmax or splits the next stage's keys.
+        // The waves w and w + 4 split at the two ends of a stage. They share a SIMD, which prefers
+        // the older one: its products run while the other splits, and the other's while it is at
+        // its softmax or splits the next stage's keys. (All at the end: 9% slower.)
         if (loads_k) {
             if (more) load_next(stage + 1);
         } else {
             if (more) stage_out(half ^ 1);
             if (stage + 2 < stages) load_next(stage + 2);
         }
-        // O's unit, from the largest values so far
-        int ke[SG], ve[SG], need = oexp;
+        int ke[SG], ve[SG];
 #pragma unroll
         for (int v = 0; v < SG; ++v) {
             ke[v] = __builtin_amdgcn_readfirstlane(exps[half][0][v]);
             ve[v] = __builtin_amdgcn_readfirstlane(exps[half][1][v]);
-            need = min(need, ve[v] + kTileTop);
         }
-        const bool lower = need != oexp;
-        const float turn0 = oexp == 1000 ? 0.f : power2(need - oexp);
-        oexp = need;
-        bool turned = !lower;
         const uint8_t* const base = lds + half * Shape::STAGE;
+        const uint32_t gx = stage * SG;
+        // wave-uniform: one of the stage's groups is visible to one of the wave's queries
+        if (!idle && gx < seen1 && (gx + SG > seen0 || gx < seen_sinks)) {
+            // scores: the small products first, so that a large sum rounds once per step
+            v16f st[2];
 #pragma unroll
-        for (int sub = 0; sub < SG / 2; ++sub) {
-            const uint32_t gx = stage * SG + 2 * sub;
-            if (idle || gx >= seen1 || (gx + 1 < seen0 && gx >= seen_sinks)) continue;  // wave-uniform
-            v16f st;
+            for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st[i] = 0.f;
-            const uint8_t* const krow = base + (32 * sub + c) * Shape::KROW + 16 * hh;
+                for (int i = 0; i < 16; ++i) st[sub][i] = 0.f;
+                const uint8_t* const krow = base + (32 * sub + c) * Shape::KROW + 16 * hh;
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                const v8h kh = *reinterpret_cast<const v8h*>(krow + 32 * j);
-                const v8h kl = *reinterpret_cast<const v8h*>(krow + Shape::KPART + 32 * j);
-                st = SL_F16(kl, qh[j], st);
-                st = SL_F16(kh, ql[j], st);
-                st = SL_F16(kh, qh[j], st);
+                for (int j = 0; j < KS; ++j) {
+                    const v8h kh = *reinterpret_cast<const v8h*>(krow + 32 * j);
+                    const v8h kl = *reinterpret_cast<const v8h*>(krow + Shape::KPART + 32 * j);
+                    st[sub] = SL_F16(kl, qh[j], st[sub]);
+                    st[sub] = SL_F16(kh, ql[j], st[sub]);
+                    st[sub] = SL_F16(kh, qh[j], st[sub]);
+                }
             }
-            if (!(gx + 1 < whole1 && (gx + 1 < whole_sinks || gx >= whole0))) {  // wave-uniform
-                const uint32_t ga = keys.group(gx), gb = keys.group(min(gx + 1, keys.groups - 1));
+            if (!(gx + SG <= whole1 && (gx + SG <= whole_sinks || gx >= whole0))) {  // wave-uniform
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t j = 16 * (i < 8 ? ga : gb) + 8 * (i / 4 % 2) + 4 * hh + i % 4;
-                    if ((i >= 8 && gx + 1 >= keys.groups) || !paged_sees(mask, g.sinks, j)) st[i] = -INFINITY;
+                for (int v = 0; v < SG; ++v) {
+                    const uint32_t key0 = 16 * keys.group(min(gx + v, keys.groups - 1)) + 4 * hh;
+                    const bool there = gx + v < keys.groups;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (!there || !paged_sees(mask, g.sinks, key0 + 8 * (i / 4) + i % 4)) st[v / 2][8 * (v % 2) + i] = -INFINITY;
                 }
             }
             // The weights are 2^(x c2 - m), x in its group's units (an exact power of two apart
             // from q.k's). m is the largest x c2, once rounded, at the time it was taken: it
             // follows only where that is kSlack beyond it, so that most tiles leave O as it is. A
             // query may see none of the keys so far (m = -inf): its weights and corr are 0.
-            const float fa = ldexpf(c2, -qe - ke[2 * sub]), fb = ldexpf(c2, -qe - ke[2 * sub + 1]);
-            float ma = fmaxf(st[0], st[1]), mb = fmaxf(st[8], st[9]);
+            float f[SG], m_new = -INFINITY;
 #pragma unroll
-            for (int i = 2; i < 8; i += 2) {
-                ma = fmaxf(fmaxf(ma, st[i]), st[i + 1]);
-                mb = fmaxf(fmaxf(mb, st[8 + i]), st[9 + i]);
+            for (int v = 0; v < SG; ++v) {
+                f[v] = ldexpf(c2, -qe - ke[v]);
+                const v16f& x = st[v / 2];
+                const int i0 = 8 * (v % 2);
+                float most = fmaxf(x[i0], x[i0 + 1]);
+#pragma unroll
+                for (int i = i0 + 2; i < i0 + 8; i += 2) most = fmaxf(fmaxf(most, x[i]), x[i + 1]);
+                m_new = fmaxf(m_new, most * f[v]);
             }
-            float m_new = fmaxf(ma * fa, mb * fb);
             m_new = fmaxf(m_new, lane_xor32(m_new));
-            if (!turned || __any(!(m_new - m <= kSlack))) {  // wave-uniform
+            if (__any(!(m_new - m <= kSlack))) {  // wave-uniform
                 m_new = fmaxf(m, m_new);
                 const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-                const float turn = turned ? corr : corr * turn0;
-                turned = true;
 #pragma unroll
-                for (int t = 0; t < DT; ++t) o[t] *= turn;
+                for (int t = 0; t < DT; ++t) o[t] *= corr;
                 l *= corr;
                 m = m_new;
                 bad |= fabsf(m) > kExponentMost && m != -INFINITY;
             }
             const float from = m == -INFINITY ? 0.f : m;
+            if (oexp >= kNoUnit) oexp = ve[0] + kTileTop;  // O is still zero
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                st[i] = __builtin_amdgcn_exp2f(fmaf(st[i], i < 8 ? fa : fb, -from));
-                l += st[i];
-            }
+            for (int v = 0; v < SG; ++v) {
+                v16f& x = st[v / 2];
+                const int i = 8 * (v % 2);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int i = 8 * s;
-                const Parts w = to_parts(st[i], st[i + 1], st[i + 2], st[i + 3], st[i + 4], st[i + 5], st[i + 6],
-                                         st[i + 7], power2(oexp - ve[2 * sub + s]));
-                const uint8_t* const vat = base + 2 * Shape::KPART + (2 * sub + s) * Shape::VGROUP + 16 * lane;
+                for (int e = i; e < i + 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], f[v], -from));
+                    l += x[e];
+                }
+                const int unit = ve[v] + kTileTop;
+                if (__builtin_expect(ve[v] != kNoUnit && (unit < oexp || unit > oexp + kUnitSlack), 0)) {  // wave-uniform
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[t][e] = __builtin_ldexpf(o[t][e], unit - oexp);
+                    oexp = unit;
+                }
+                const Parts w = to_parts(x[i], x[i + 1], x[i + 2], x[i + 3], x[i + 4], x[i + 5], x[i + 6], x[i + 7],
+                                         power2(oexp - ve[v]));
+                const uint8_t* const vat = base + 2 * Shape::KPART + v * Shape::VGROUP + 16 * lane;
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
                     const v8h vh = *reinterpret_cast<const v8h*>(vat + (2 * t) * 1024);
@@ -309,17 +353,14 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
                 }
             }
         }
-        if (!turned) {  // no keys of the stage for this wave, but another unit
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[t] *= turn0;
-        }
         if (loads_k && more) stage_out(half ^ 1);
         __syncthreads();
     }
 #undef SL_F16
     // (the arguments again from here on: kept through the loop they would cost it registers)
     const PagedGeo e = geometry_again();
-    const float back = oexp == 1000 ? 0.f : power2(-oexp);
+    const bool direct = paged_direct(e);
+    const float back = oexp >= kNoUnit ? 0.f : power2(-oexp);
     float check = l;
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
@@ -336,7 +377,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
     const uint32_t mine_here = count > 32u * wave ? min(count - 32u * wave, 32u) : 0;  // the wave's query rows
     if (!__any(bad)) {  // wave-uniform
         // the wave's rows through LDS, so that they are written whole
-        const float f = e.slots == 1 ? 1.0f / l : 1.f;
+        const float f = direct ? 1.0f / l : 1.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float* const to = so + c * OROW + VW * (8 * (i / 4) + 4 * hh + i % 4);
@@ -345,7 +386,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
             else *reinterpret_cast<float2*>(to) = make_float2(o[0][i] * f, o[1][i] * f);
         }
         const uint32_t d4 = D / 4;
-        const bool al = e.slots != 1 || aligned;
+        const bool al = !direct || aligned;
         const auto place_of = [&](uint32_t x) {
             const uint32_t rr = it.r0 + 32u * wave + x;
             return static_cast<uint64_t>(it.t0 + rr / G) * e.heads + kvh * G + rr % G;
@@ -354,10 +395,10 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
             const uint32_t x = i / d4, d = 4 * (i % d4);
             const float4 v = *reinterpret_cast<const float4*>(so + x * OROW + d);
             const uint64_t to = place_of(x);
-            store4(e.slots == 1 ? e.out + to * D + d : e.part + (to * e.slots + it.slot) * D + d, v, al);
+            store4(direct ? e.out + to * D + d : e.part + (to * e.slots + it.slot) * D + d, v, al);
         }
-        if (e.slots != 1 && static_cast<uint32_t>(lane) < mine_here)  // (lanes c of the lower half: query c)
-            e.ml[place_of(lane) * e.slots + it.slot] = make_float2(m, l);
+        if (static_cast<uint32_t>(lane) < mine_here)  // (lanes c of the lower half: query c)
+            paged_state(e, it, place_of(lane), m, l);
         return;
     }
     // Values that are not finite somewhere: the wave's queries again, in f32, 16 at a time.
@@ -371,17 +412,17 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
         l += lane_xor16(l);
         l += lane_xor32(l);
         if (q0 + lane % 16 >= count) continue;
-        const float f = e.slots == 1 ? 1.0f / l : 1.f;
-        float* const d0 = e.slots == 1 ? e.out + to * D : e.part + (to * e.slots + it.slot) * D;
+        const float f = direct ? 1.0f / l : 1.f;
+        float* const d0 = direct ? e.out + to * D : e.part + (to * e.slots + it.slot) * D;
         for (uint32_t d = lane / 16; d < D; d += 4) d0[d] = own[d] * f;
-        if (e.slots != 1 && lane < 16) e.ml[to * e.slots + it.slot] = make_float2(m, l);
+        if (lane < 16) paged_state(e, it, to, m, l);
     }
 }
 
 }  // namespace
 
-hipError_t launch_paged_tiles(const PagedGeo& g, uint64_t items, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(items * g.kv_heads), g.shared_items ? g.shared_splits : g.splits);
+hipError_t launch_paged_tiles(const PagedGeo& g, hipStream_t s) {
+    const unsigned grid = paged_blocks(g);
     const bool exact = g.head_dim % 64 == 0;
     if (g.head_dim <= 64) {
         if (exact) paged_tiles<1, true><<<grid, 64 * NW, 0, s>>>(g);

@@ -66,7 +66,8 @@ bool check_paged_call(const BufferView& buffers, const PagedCall& given, Error* 
     if (kv.num_pages == 0 || kv.pages_per_seq == 0) return fail(err, Error::execution("the page pool is empty"));
     if (product({kv.pages_per_seq, kv.page_size}) > kPositionsMost)
         return fail(err, Error::unimplemented("a block table covers more than 2^31 - 1 positions"));
-    if (product({T, H}) > kPositionsMost || product({B, Hkv}) > (1u << 26))
+    // (the launches' threads, at most (T H / 16 + B Hkv) 512 and 256 T, are counted in 32 bits)
+    if (T >= 1u << 24 || product({T, H}) > 1u << 25 || product({B, Hkv}) > 1u << 22)
         return fail(err, Error::unimplemented("too many tokens or rows for one call"));
     const auto kind_of = [&](uint32_t id) -> uint32_t {
         const sl_buffer_desc* d = buffers.get(id);
@@ -134,13 +135,13 @@ bool check_paged_contents(const PagedCall& c, const PagedTables& t, uint32_t few
     };
     const auto pages = [&](uint64_t positions) { return (positions + ps - 1) / ps; };
     const char* const bad_id = "page id out of range";
-    uint64_t keys = 0;
     const uint64_t group = c.op->heads / c.op->kv_heads;
     const uint32_t* shared = nullptr;  // the prefix's pages
     for (uint64_t b = 0; b < B; ++b) {
         const uint64_t L = t.seq_lens[b], n = starts[b + 1] - starts[b], end = L + n;
         if (n == 0) continue;
         const uint64_t rows = n * group;
+        uint64_t keys = 0;  // that the row's queries see at most
         plan->rows_with_tokens += 1;
         if (rows <= few) plan->few_rows += (rows + 15) / 16 * 16;  // (each row's blocks counted up)
         else plan->many_rows += (rows + 15) / 16 * 16, plan->many_blocks += (rows + 255) / 256;
@@ -155,7 +156,7 @@ bool check_paged_contents(const PagedCall& c, const PagedTables& t, uint32_t few
             }
             if (!in_range(b, first / ps, pages(end)) || !in_range(b, 0, pages(sinks)))
                 return fail(err, Error::execution(bad_id));
-            keys = std::max(keys, end - first + sinks);
+            keys = end - first + sinks;
         } else {
             if (L < c.prefix) return fail(err, Error::execution("a row is shorter than the shared prefix"));
             const uint32_t* const ids = t.block_table + b * per;
@@ -166,8 +167,11 @@ bool check_paged_contents(const PagedCall& c, const PagedTables& t, uint32_t few
                 return fail(err, Error::execution("a row does not begin with the shared prefix's pages"));
             }
             if (!in_range(b, c.prefix / ps, pages(end))) return fail(err, Error::execution(bad_id));
-            keys = std::max(keys, end);
+            keys = end;
         }
+        uint32_t& most = rows <= few ? plan->few_keys : plan->many_keys;
+        most = std::max(most, static_cast<uint32_t>(keys));
+        (rows <= few ? plan->few_keys_in_all : plan->many_keys_in_all) += keys;
     }
     if (c.kind == SL_PAGED_APPEND && T != 0) {
         // A page that a row writes belongs to that row alone: neither another row's
@@ -197,7 +201,6 @@ bool check_paged_contents(const PagedCall& c, const PagedTables& t, uint32_t few
             if (hit) return fail(err, Error::execution(twice));
         }
     }
-    plan->most_keys = static_cast<uint32_t>(keys);
     return true;
 }
 

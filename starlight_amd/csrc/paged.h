@@ -29,9 +29,11 @@ struct PagedCall {
 
 // What the launch is sized for.
 struct PagedPlan {
-    uint32_t most_keys = 0;  // the most keys that one row's queries see
-    // query rows per KV head of the rows with up to `few` of them, of the others, and the others'
-    // blocks of 256 (each row's counted up); rows with tokens
+    // The most keys that one row's queries see, and the query rows per KV head (each row's counted
+    // up to whole blocks), of the rows with up to `few` query rows and of the others; the others'
+    // blocks of 256; rows with tokens.
+    uint32_t few_keys = 0, many_keys = 0;
+    uint64_t few_keys_in_all = 0, many_keys_in_all = 0;
     uint64_t few_rows = 0, many_rows = 0, many_blocks = 0, rows_with_tokens = 0;
 };
 
