@@ -12,15 +12,18 @@ from starlight_amd.paged import PAGE_NONE
 pytestmark = pytest.mark.gpu
 
 
-def large_row(window, group):
-    """(cached, new) tokens of a row that makes a call large: 6,400 query rows per
-    KV head behind a window, 1,600 that see 2,600 keys without."""
-    return (300, 6400 // group) if 0 < window <= 500 else (2600, 1600 // group)
+def large_row(window, heads, kv_heads):
+    """(cached, new) tokens of a row that makes a call large: 32,000 queries (tokens times heads)
+    behind a short window, 8,000 behind a longer one, and without one 1,600 per KV head that see
+    2,600 keys and more."""
+    if window == 0 or window > 2600:
+        return 2600, 1600 * kv_heads // heads
+    return (300, 32000 // heads) if window <= 500 else (2600, 8000 // heads)
 
 
 def call(hip, rng, heads, kv_heads, dim, lens, news, page=16, window=0, layers=1, layer=0):
     """Rows of the given lengths with a large one in their midst."""
-    past, new = large_row(window, heads // kv_heads)
+    past, new = large_row(window, heads, kv_heads)
     at = len(lens) // 2
     return Rows(hip, rng, heads, kv_heads, dim, lens[:at] + [past] + lens[at:], news[:at] + [new] + news[at:], page,
                 layers=layers, layer=layer)
@@ -67,19 +70,17 @@ def test_page_sizes(hip, page, window):
     check(call(hip, rng, 8, 2, 128, [0, 95, 333], [70, 1, 17], page, window), window, 5)
 
 
-@pytest.mark.parametrize("batch", [63, 64, 65, 150])
-@pytest.mark.parametrize("large", [0, 60, -1])
+@pytest.mark.parametrize("batch,large", [(63, 0), (64, -1), (65, 60), (65, -1), (150, 0), (150, 100)])
 def test_many_rows(hip, batch, large):
     """The large row among the first 64 rows and behind them."""
     rng = np.random.default_rng(batch)
     lens = [int(x) for x in rng.integers(0, 100, batch)]
     news = [int(x) for x in rng.choice([0, 1, 3, 40, 70], batch)]
-    lens[large], news[large] = large_row(40, 4)
+    lens[large], news[large] = large_row(40, 4, 1)
     check(Rows(hip, rng, 4, 1, 64, lens, news), 40, 2)
 
 
-@pytest.mark.parametrize("offset", [1, 2, 3, 4])
-@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("offset,dim", [(1, 64), (2, 128), (3, 80), (4, 48)])
 def test_ports_at_any_offset(hip, offset, dim):
     rng = np.random.default_rng(offset)
     check(call(hip, rng, 8, 2, dim, [40, 300], [3, 50], window=100), 100, 4, offset=offset)
@@ -192,8 +193,7 @@ def test_large_values_of_unseen_keys_do_not_matter(hip, factor, dim, large):
 
 
 @pytest.mark.parametrize("factor", FACTORS)
-@pytest.mark.parametrize("dim", [64, 128, 80, 192])
-@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("dim,large", [(64, False), (64, True), (128, False), (128, True), (80, True), (192, False)])
 def test_one_large_column(hip, factor, dim, large):
     """One dimension of the values far larger than the others."""
     rng = np.random.default_rng(10)
@@ -205,8 +205,7 @@ def test_one_large_column(hip, factor, dim, large):
     check(rows, 100 if large else 20)
 
 
-@pytest.mark.parametrize("dim", [64, 128, 192])
-@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("dim,large", [(64, False), (64, True), (128, False), (128, True), (48, True), (192, False)])
 def test_zeros_among_the_keys(hip, dim, large):
     """Rows of zeros, as a cleared cache holds, and whole pages of them."""
     rng = np.random.default_rng(11)
