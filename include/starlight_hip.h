@@ -343,8 +343,8 @@ typedef struct sl_paged_tokens {
  * and stores the new keys and values, then one of the two attentions reads them.
  * `op` is the layer's CausalAttention op (layer, heads, kv_heads, head_dim, scale;
  * head_dim a multiple of 16 up to 256, up to 1024 heads, any number of query heads
- * per KV head);
- * q, k, v and outputs are token-major, [tokens, heads, head_dim] and [tokens,
+ * per KV head); a call has up to 2^24 - 1 tokens, 2^25 tokens times heads and 2^22
+ * rows times KV heads. q, k, v and outputs are token-major, [tokens, heads, head_dim] and [tokens,
  * kv_heads, head_dim], f32 at any offset, as projections write and read them.
  * The tables, lengths and row starts are checked on the host from the last
  * upload_u32. Each call submits the logged commands first and enqueues its
@@ -355,16 +355,17 @@ typedef struct sl_paged_tokens {
  * still satisfy what is said here, with the same number of tokens. seq_lens is
  * not advanced: the caller adds each row's tokens after the step. Errors beside
  * those named: UnsupportedOp for another op code; Unimplemented for a head_dim,
- * heads or page_size not named here, buffers above 16 MiB, or a block table of more
- * than 2^31 - 1 positions; Execution for shapes, lengths, row starts, page ids
+ * heads, page_size or number of tokens and rows not named here, buffers above 16 MiB,
+ * or a block table of more than 2^31 - 1 positions; Execution for shapes, lengths, row starts, page ids
  * or aliases that do not fit; InvalidBuffer and InvalidRange as dispatch. A
  * refused call changes nothing. */
 
 /* Stores the new keys and values k and v at their positions in layer op->layer
  * of the cache, the keys rotated as the Rope op `rope` (variant, theta) rotates
  * them at those positions, or as they are when rope is null. q and q_out, both
- * or neither: the queries, rotated the same way. Rotated values equal the Rope
- * operator's bit for bit. Execution when a page that a row appends into is also
+ * or neither: the queries, rotated the same way. Rotated values are the Rope
+ * operator's (angles, sines and cosines in f64, rounded once), but for a last bit
+ * where the f64 sines differ, about once in 2^28 values. Execution when a page that a row appends into is also
  * another row's, or twice the row's own. */
 sl_status sl_hip_paged_append(sl_hip_device *device, const sl_op *op, const sl_op *rope, const sl_buffer_ref *q,
                               const sl_buffer_ref *k, const sl_buffer_ref *v, const sl_buffer_ref *q_out,
@@ -374,7 +375,11 @@ sl_status sl_hip_paged_append(sl_hip_device *device, const sl_op *op, const sl_o
  * (already appended) included: a token at position p sees the positions j <= p
  * with j > p - window or j < sinks; window 0 is no window, and sinks is then not
  * read. Pages without a position that a token of the call sees are not read, and
- * their table entries may be anything. */
+ * their table entries may be anything. Accurate as f32 sums are: operands are two
+ * fp16 parts each, 22 bits of the largest of a block of 16 or 32 positions. Blocks
+ * whose positions (or, of the values, dimensions) lie 2^16 apart, and values that are
+ * not finite, take a plain f32 form, many times slower. What a token does not see
+ * never reaches its result. */
 sl_status sl_hip_paged_window_attention(sl_hip_device *device, const sl_op *op, const sl_buffer_ref *q,
                                         const sl_buffer_ref *out, uint32_t window, uint32_t sinks,
                                         const sl_paged_tokens *tokens, const sl_paged_kv *kv);
@@ -389,9 +394,9 @@ sl_status sl_hip_paged_prefix_attention(sl_hip_device *device, const sl_op *op, 
                                         const sl_paged_kv *kv);
 
 /* The device address of f32 buffer `buffer`, valid until the device is destroyed,
- * and, where `elements` is not null, its capacity: for a program that makes or reads its contents with kernels of its own, or hands
- * them to another library without a copy (no reference counterpart). Logged
- * commands are submitted first; accesses are ordered with the device's work as any
+ * and, where `elements` is not null, its capacity: for a program that makes or reads
+ * its contents with kernels of its own, or hands them to another library without a
+ * copy (no reference counterpart). Logged commands are submitted first; accesses are ordered with the device's work as any
  * other on sl_hip_stream's device are (on that stream, or synchronized). Writing
  * the scales of a bound quantized weight this way does not refresh its copies.
  * InvalidBuffer for a u32 buffer, whose contents the device also keeps on the

@@ -292,3 +292,20 @@ def test_tokens_of_more_rows_than_there_are():
         with pytest.raises(ValueError):
             t.set(bad)
     assert device.PAGED_PREFIX == 2
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens,batch,heads,refused", [
+    ((1 << 25) // H, 3, H, False), ((1 << 25) // H + 1, 3, H, True),
+    ((1 << 24) - 1, 3, 1, False), (1 << 24, 3, 1, True),
+    (5, (1 << 22) // HKV, H, False), (5, (1 << 22) // HKV + 1, H, True)])
+def test_what_the_launches_can_count(kind, tokens, batch, heads, refused):
+    """The limits themselves: one below is refused for the buffers' sizes, which a call
+    of that size would need."""
+    c = Call(kind)
+    c.op = Op.causal_attention(1, heads, min(heads, HKV), D, 0.125)
+    c.tokens.update(tokens=tokens, batch=batch)
+    c.buffers[0]["elements"] = 2 * 12 * 2 * 16 * min(heads, HKV) * D
+    error = c.run()
+    assert (error == DeviceError.unimplemented("too many tokens or rows for one call")) == refused
+    assert error is not None
