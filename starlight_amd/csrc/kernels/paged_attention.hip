@@ -319,7 +319,7 @@ __global__ __launch_bounds__(64 * NW, DV <= 2 ? 2 : 1) void paged_rows(PagedGeo 
             if (f != 0.f) fma4(acc, f, *reinterpret_cast<const float4*>(&so[w][x][d]));
         }
         const uint64_t at = row_of(it.r0 + x);
-        if (paged_direct(g)) store4(g.out + at * D + d, scaled4(acc, 1.0f / sum), aligned);
+        if (paged_direct(g, it)) store4(g.out + at * D + d, scaled4(acc, 1.0f / sum), aligned);
         else *reinterpret_cast<float4*>(g.part + (at * g.slots + it.slot) * D + d) = acc;
         if (d == 0) paged_state(g, it, at, mm, sum);
     }
@@ -356,8 +356,10 @@ __global__ __launch_bounds__(256) void paged_merge(PagedGeo g) {
     uint32_t count = S;  // the row's partials
     if (g.uneven != 0) {
         for (count = 0; count < S && !(ml[x][count].y < 0.f);) ++count;
-        last = max(count, 1u) - 1;
-        load(0);
+        if (count != 0) {
+            last = count - 1;
+            load(0);
+        }
     }
     for (uint32_t s = 0; s < count; ++s) mm = fmaxf(mm, ml[x][s].x);
     __syncthreads();
@@ -411,7 +413,7 @@ PagedGeo paged_geometry(const PagedTokensArgs& a) {
     g.num_pages = a.num_pages;
     g.window = a.window == 0 ? 0xffffffffu : a.window;
     g.sinks = a.window == 0 ? 0 : a.sinks;
-    g.splits = g.slots = 1;
+    g.splits = g.slots = g.tail_splits = 1;
     g.aligned = aligned16(a.q) && aligned16(a.out);
     g.rows_upto = 0xffffffffu;
     g.scale = a.scale;
@@ -537,13 +539,28 @@ hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hi
             few = rows_splits(g, a.few_rows, most_few, a.few_keys);
             few.us = std::max(few.us, read_us(g, a.few_keys_in_all));
         }
-        ts = tiles_splits(g, a.many_blocks, t.own_items, seen(a.many_keys, kTileRows));
+        const uint64_t keys = seen(a.many_keys, kTileRows);
+        ts = tiles_splits(g, a.many_blocks, t.own_items, keys);
+        // Not split, but the last round of blocks less than half full: those blocks alone. (376 blocks
+        // of a prompt of 3,001 of the 1B shape: 134 -> 119 us.)
+        const uint32_t round = static_cast<uint32_t>(compute_units()) / g.kv_heads;
+        const uint32_t rest = round != 0 ? a.many_blocks % round : 0;
+        if (ts.n == 1 && a.many_blocks > round && rest != 0 && 2 * rest <= round) {
+            const Splits last = tiles_splits(g, rest, rest, keys);
+            const double us = kTilesCosts.step_us * (a.many_blocks / round) *
+                                  (static_cast<double>((keys + 63) / 64) + kTilesCosts.fixed) + last.us;
+            if (last.n > 1 && us < ts.us) {
+                t.round_items = round;
+                t.tail_splits = last.n;
+                ts.us = us;
+            }
+        }
         if (few.us + ts.us < std::max(rs.us, read_us(g, a.few_keys_in_all + a.many_keys_in_all))) {
             rs = few;
             tiles = true;
             some = a.few_rows != 0;
         } else {
-            ts.n = 1;
+            ts.n = t.tail_splits = 1;
         }
         if (tiles && some) {
             r.rows_upto = t.rows_over = kPagedFewRows;
@@ -553,14 +570,18 @@ hipError_t launch_paged_window(const PagedTokensArgs& a, const Workspace& ws, hi
     // (as many splits as the workspace has room for)
     const uint64_t room = ws.floats / (static_cast<uint64_t>(g.tokens) * g.heads * (g.head_dim + 2) + 64);
     const auto fit = [&](uint32_t n) { return static_cast<uint32_t>(std::min<uint64_t>(n, std::max<uint64_t>(room, 1))); };
-    const uint32_t slots = fit(std::max(rs.n, ts.n));
+    const uint32_t slots = fit(std::max({rs.n, ts.n, t.tail_splits}));
+    t.tail_splits = fit(t.tail_splits);
     if (slots > 1 && place_partials(&g, slots, ws)) {
         r.splits = fit(rs.n);
         t.splits = fit(ts.n);
-        g.uneven = some && tiles && r.splits != t.splits;
+        g.uneven = t.tail_splits > 1 || (some && tiles && r.splits != t.splits);
+        if (t.tail_splits > 1) t.own_items += t.round_items * (t.tail_splits - 1);
         r.slots = t.slots = slots;
         r.ml = t.ml = g.ml;
         r.part = t.part = g.part;
+    } else {
+        t.tail_splits = 1;
     }
     hipError_t e = hipSuccess;
     if (some) e = launch_rows(r, s);

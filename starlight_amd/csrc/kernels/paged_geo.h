@@ -32,8 +32,10 @@ struct PagedGeo {
     // shared_splits, all tokens' queries over the positions below `prefix`, which lie in the same
     // pages for every row.
     uint32_t prefix, shared_items, shared_splits, own_items, splits;
+    // Own items in whole rounds of round_items, the rest of them split by tail_splits (1: not).
+    uint32_t round_items, tail_splits;
     // Partials a query row has room for, the shared first. A row that leaves the later of
-    // them ends its list with a sum of -1 (splits 1 and no prefix: at once, its result is written).
+    // them ends its list with a sum of -1 (not split and no prefix: at once, its result is written).
     uint32_t slots;
     uint32_t uneven;                            // rows have fewer partials than slots
     uint32_t aligned;                           // q and out are 16-byte aligned
@@ -131,11 +133,21 @@ __device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t unit, uin
     PagedRow r = paged_row(g, 0, M);
     uint32_t x = unit, first = 0;
     it->split = 0;
+    it->splits = g.splits;
     if (LAST_FIRST || g.splits != 1) {
         uint32_t total = paged_row_items(r);
         for (uint32_t b0 = kWave; b0 < g.batch; b0 += kWave) total += paged_row_items(paged_row(g, b0, M));
-        if (unit >= total * g.splits) return false;
-        if (g.splits != 1) {
+        if (LAST_FIRST && g.tail_splits > 1) {
+            const uint32_t tail = total % g.round_items, whole = total - tail;
+            if (unit >= whole + tail * g.tail_splits) return false;
+            if (unit >= whole) {
+                it->splits = g.tail_splits;
+                it->split = (unit - whole) / tail;
+                x -= it->split * tail;
+            }
+        } else if (unit >= total * g.splits) {
+            return false;
+        } else if (g.splits != 1) {
             it->split = unit / total;
             x -= it->split * total;
         }
@@ -151,7 +163,6 @@ __device__ __forceinline__ bool paged_item(const PagedGeo& g, uint32_t unit, uin
     const int at = __builtin_ctzll(found);
     it->begin = g.prefix;
     it->end = 0xffffffffu;
-    it->splits = g.splits;
     it->slot = (g.prefix != 0 ? g.shared_splits : 0) + it->split;
     it->b = first + at;
     it->t0 = __builtin_amdgcn_readlane(r.start, at);
@@ -183,18 +194,20 @@ __device__ __forceinline__ PagedKeys paged_keys(const PagedGeo& g, const PagedIt
     return k;
 }
 
-// Whether the launch writes results, not partials.
-__device__ __forceinline__ bool paged_direct(const PagedGeo& g) { return g.splits == 1 && g.prefix == 0; }
+// Whether the item's results are written, not partials.
+__device__ __forceinline__ bool paged_direct(const PagedGeo& g, const PagedItem& it) {
+    return it.splits == 1 && g.prefix == 0;
+}
 // The partial `slot` of a query row (token and head), its values written by the caller; `m` and
 // `l` are not looked at for a result.
 __device__ __forceinline__ void paged_state(const PagedGeo& g, const PagedItem& it, uint64_t row, float m, float l) {
     float2* const ml = g.ml + row * g.slots;
-    if (paged_direct(g)) {
+    if (paged_direct(g, it)) {
         if (g.slots > 1) ml[0] = make_float2(0.f, -1.f);
         return;
     }
     ml[it.slot] = make_float2(m, l);
-    if (g.prefix == 0 && it.split == 0 && g.splits < g.slots) ml[g.splits] = make_float2(0.f, -1.f);
+    if (g.prefix == 0 && it.split == 0 && it.splits < g.slots) ml[it.splits] = make_float2(0.f, -1.f);
 }
 
 // Which keys a query at `position` sees: j < end and (j >= low or j < sinks).
@@ -221,6 +234,22 @@ __device__ __forceinline__ PagedGeo geometry_again() {
 #pragma unroll
     for (size_t i = 0; i < sizeof(PagedGeo) / 8; ++i) words.w[i] = p[i];
     return __builtin_bit_cast(PagedGeo, words);
+}
+
+// Which keys an item takes, in one register through a kernel's loop, and again from it. (In six,
+// more of the loop's were spilled: 1.5% of paged_tiles. All that its end needs in LDS: 1%.)
+__device__ __forceinline__ uint32_t paged_pack(const PagedItem& it) {
+    uint32_t part = it.slot | it.split << 8 | it.splits << 16 | (it.end != 0xffffffffu ? 1u << 31 : 0);
+    asm volatile("" : "+s"(part));
+    return part;
+}
+__device__ __forceinline__ void paged_unpack(const PagedGeo& g, uint32_t part, PagedItem* it) {
+    const bool shared = part >> 31 != 0;
+    it->slot = part & 255;
+    it->split = part >> 8 & 255;
+    it->splits = part >> 16 & 255;
+    it->begin = shared ? 0 : g.prefix;
+    it->end = shared ? g.prefix : 0xffffffffu;
 }
 
 // Word i of a table that no kernel writes, the same for the whole wave: a scalar load.

@@ -25,8 +25,8 @@
 // 11,000 cycles where its products take 6,100. 2,048 tokens at 6,000 of the 8B shape behind
 // a window of 4,096: 410 us, 1.0 PFLOP/s of fp16 products, three of them per product
 // (hipBLASLt's 8192^3 reaches 1.08). The scores of a whole stage before its softmax, not of
-// 32 keys at a time: 128 us, not 132, for a prompt of 3,001 of the 1B shape, and 134 with the
-// looks at how far the rows and groups lie apart.
+// 32 keys at a time: 128 us, not 132, for a prompt of 3,001 of the 1B shape; 134 with the
+// looks at how far the rows and groups lie apart; 119 with its last round's blocks split.
 // No better: two tiles of 32 queries per wave, blocks of 4 waves, stages of 32 keys, raised wave
 // priorities; four waves per SIMD at head_dim 64 spill and take 160 us for that prompt.
 #include "paged_geo.h"
@@ -88,6 +88,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
     const float* const qrow = g.q + (static_cast<uint64_t>(it.t0 + r / G) * g.heads + kvh * G + r % G) * D;
     const uint64_t row = static_cast<uint64_t>(g.kv_heads) * D;
     const bool aligned = g.aligned != 0;
+    const uint32_t part = paged_pack(it);
     if (tid == 0) flags = 0;
     __syncthreads();
 
@@ -359,7 +360,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tiles(PagedGeo g) {
 #undef SL_F16
     // (the arguments again from here on: kept through the loop they would cost it registers)
     const PagedGeo e = geometry_again();
-    const bool direct = paged_direct(e);
+    paged_unpack(e, part, &it);
+    const bool direct = paged_direct(e, it);
     const float back = oexp >= kNoUnit ? 0.f : power2(-oexp);
     float check = l;
 #pragma unroll

@@ -8,6 +8,7 @@ import pytest
 from paged_tokens import Rows, assert_within, attention64, read_port
 from starlight_amd.ir import Op
 from starlight_amd.paged import PAGE_NONE
+from test_gpu_paged_serving import Graph
 
 pytestmark = pytest.mark.gpu
 
@@ -220,3 +221,44 @@ def test_zeros_among_the_keys(hip, dim, large):
                 rows.pool[0, p, 0, s] = 0
     rows.upload()
     check(rows, 100 if large else 0)
+
+
+# prompts of a whole round of blocks of 256 query rows and part of another (32 and 128 of
+# each KV head's fill 256 CUs): the part is split over the keys
+@pytest.mark.parametrize("heads,kv_heads,dim,new", [(32, 8, 64, 2400), (32, 8, 128, 2100), (8, 2, 64, 8300),
+                                                    (8, 2, 112, 9000)])
+@pytest.mark.parametrize("lens,news", [([], []), ([900, 3, 0], [1, 70, 2])])
+def test_the_last_round_of_blocks(hip, heads, kv_heads, dim, new, lens, news):
+    rng = np.random.default_rng(new)
+    check(Rows(hip, rng, heads, kv_heads, dim, lens[:1] + [70] + lens[1:], news[:1] + [new] + news[1:]), 150, 4)
+
+
+def test_the_last_round_changes_between_replays(hip):
+    """Captured for a prompt whose last round of blocks is split; replayed with its
+    tokens in rows of other numbers, so that more, fewer or no blocks are left over."""
+    rng = np.random.default_rng(12)
+    news = [[2400, 0, 1], [1100, 1300, 1], [1, 2048, 352], [3, 2046, 352], [2394, 7, 0]]
+    lens = [[30, 0, 500], [10, 600, 0], [900, 0, 3], [0, 0, 0], [5, 300, 0]]
+    most = [max(l[b] + n[b] for l, n in zip(lens, news)) for b in range(3)]
+    rows = Rows(hip, rng, 32, 8, 64, [m - 1 for m in most], [1] * 3)
+    q = (rng.standard_normal((2401, 32, 64)) * 2).astype(np.float32)
+    op = Op.causal_attention(0, 32, 8, 64, 0.125)
+    qr, out = rows.buffer(q), rows.buffer(np.zeros_like(q))
+
+    def put(i):
+        rows.lens, rows.news = lens[i], news[i]
+        hip.upload_u32(rows.cache.lens_buffer, np.asarray(rows.lens, np.uint32))
+        rows.tokens.set(rows.news)
+
+    put(0)
+    graph = Graph(hip, lambda: rows.cache.window_attention(op, rows.tokens, qr, out, 150, 4))
+    try:
+        for i in (0, 1, 2, 3, 4, 0):
+            put(i)
+            want, bound = attention64(rows, q, 0.125, 150, 4)
+            graph.launch()
+            assert_within(read_port(hip, out, q.shape), want, bound)
+            rows.cache.window_attention(op, rows.tokens, qr, out, 150, 4)
+            assert_within(read_port(hip, out, q.shape), want, bound)
+    finally:
+        graph.close()
