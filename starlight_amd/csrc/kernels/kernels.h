@@ -232,6 +232,9 @@ struct RopePowers {
 };
 hipError_t launch_paged_append(const PagedAppendArgs& a, const RopePowers& powers, hipStream_t s);
 
+// Query rows per KV head up to which a row keeps to paged_rows in a call whose others are
+// paged_tiles'. (8B shape, 4 rows of 8 tokens at 16,000: 120 us, with 16 here 146; 12 rows of 1 to
+// 300 tokens: 89.8 and 88.0.)
 constexpr uint32_t kPagedFewRows = 32;
 struct PagedTokensArgs {
     const uint32_t* starts;

@@ -252,3 +252,16 @@ def test_rows_change_their_kind_between_replays(hip):
             assert_within(read_port(hip, out, q.shape), want, bound)
     finally:
         graph.close()
+
+
+@pytest.mark.parametrize("batch", [64, 65, 130])
+@pytest.mark.parametrize("news", [{-1: 1}, {0: 1, -1: 3}, {3: 2, 63: 1}, {60: 40, -1: 1}])
+def test_long_rows_among_many_that_sit_out(hip, batch, news):
+    """A few long rows, split over their keys, anywhere in a large batch whose others
+    have no tokens."""
+    rng = np.random.default_rng(batch)
+    lens, counts = [0] * batch, [0] * batch
+    for b, n in news.items():
+        lens[b], counts[b] = 5000 + 100 * n, n
+    check_window(Rows(hip, rng, 8, 2, 64, lens, counts))
+    check_window(Rows(hip, rng, 8, 2, 64, lens, counts), 3000, 20)
